@@ -1,5 +1,5 @@
-"""ctypes binding of libnabla_optim.so (the C ABI of include/nabla_optim.h and, for
-measurement, include/nabla_optim_bench.h).
+"""ctypes binding of libnabla_optim.so (the C ABI of include/nabla_optim.h, of the operators in
+include/nabla_ops.h and, for measurement, include/nabla_optim_bench.h).
 
 The library is the product; there is no Python or CPU fallback.  If the shared
 object is missing, or no gfx950 device can be initialised, importing is still
@@ -36,6 +36,7 @@ KIND_ADAMW, KIND_ADAM, KIND_SGD = 0, 1, 2
 STEP_ZERO_GRADS = 1
 STEP_SKIP_NONFINITE = 2
 STEP_ZERO_ON_SKIP = 4
+ID_I32, ID_I64 = 0, 1
 ACC_CHECK_FINITE = 1
 ACC_WRITE_GRADS = 2
 
@@ -71,6 +72,26 @@ class StepInfo(C.Structure):
         ("step_count", C.c_uint64),
         ("found_inf", C.c_uint32),
         ("clipped", C.c_uint32),
+    ]
+
+
+class Matrix(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("rows", C.c_uint64),
+        ("cols", C.c_uint64),
+        ("stride", C.c_uint64),
+        ("dtype", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class Ids(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("n", C.c_uint64),
+        ("type", C.c_int32),
+        ("reserved", C.c_int32),
     ]
 
 
@@ -138,6 +159,20 @@ SYMBOLS = {
                                                C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_char_p),
                                                C.c_char_p]),
 }
+# every symbol include/nabla_ops.h declares
+_MP, _IP = C.POINTER(Matrix), C.POINTER(Ids)
+OPS_SYMBOLS = {
+    "nbo_embedding": (C.c_int, [_MP, _IP, _MP, C.c_double, _MP]),
+    "nbo_embedding_ws_create": (C.c_int, [C.c_uint64, C.c_uint64, C.POINTER(_P)]),
+    "nbo_embedding_ws_destroy": (C.c_int, [_P]),
+    "nbo_embedding_grad": (C.c_int, [_MP, _IP, C.c_double, C.c_int, _MP, _P]),
+    "nbo_rng_create": (C.c_int, [C.c_uint64, C.c_uint64, C.POINTER(_P)]),
+    "nbo_rng_destroy": (C.c_int, [_P]),
+    "nbo_rng_state_get": (C.c_int, [_P, _U64P, _U64P]),
+    "nbo_rng_load_state": (C.c_int, [_P, C.c_uint64, C.c_uint64]),
+    "nbo_rng_advance": (C.c_int, [_P, C.c_uint64]),
+    "nbo_dropout": (C.c_int, [_MP, _MP, C.c_double, _P, C.c_uint32, _MP]),
+}
 # every symbol include/nabla_optim_bench.h declares (measurement only)
 BENCH_SYMBOLS = {
     "nbo_copy_bytes": (C.c_int, [_P, _P, C.c_uint64]),
@@ -189,7 +224,7 @@ def load() -> C.CDLL:
     except ImportError:
         pass
     lib = C.CDLL(LIB_PATH)
-    for name, (restype, argtypes) in list(SYMBOLS.items()) + list(BENCH_SYMBOLS.items()):
+    for name, (restype, argtypes) in list(SYMBOLS.items()) + list(OPS_SYMBOLS.items()) + list(BENCH_SYMBOLS.items()):
         fn = getattr(lib, name)  # AttributeError if the library lacks a declared symbol
         fn.restype = restype
         fn.argtypes = argtypes

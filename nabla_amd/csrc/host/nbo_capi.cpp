@@ -17,6 +17,44 @@ std::recursive_mutex &api_mutex()
     static std::recursive_mutex m;
     return m;
 }
+
+// A kernel that is handed a host address, or a shape larger than the allocation behind the
+// address, faults the GPU -- which can take the whole machine's GPUs down with it -- so every
+// tensor is checked against what the HIP runtime knows about its address before a list is
+// (re)bound: the address must be device-accessible memory the runtime has allocated or
+// registered, and the tensor must end inside that allocation.  (An allocator that hands out
+// pieces of a larger block is only checked against the block.)  NBO_CHECK_POINTERS=0 in the
+// environment skips the check.
+bool pointer_checks_enabled()
+{
+    static const bool on = [] {
+        const char *v = std::getenv("NBO_CHECK_POINTERS");
+        return !(v && v[0] == '0' && v[1] == '\0');
+    }();
+    return on;
+}
+
+void check_device_address(const void *ptr, uint64_t bytes, const char *what)
+{
+    char where[96];
+    std::snprintf(where, sizeof(where), "%s at %p", what, ptr);
+    hipPointerAttribute_t attr;
+    const hipError_t e = hipPointerGetAttributes(&attr, ptr);
+    if (e != hipSuccess) (void)hipGetLastError();
+    if (e != hipSuccess || attr.type == hipMemoryTypeUnregistered)
+        fail(NBO_ERR_ARG, std::string(where) + ": not memory the HIP runtime knows (a host pointer?)");
+    hipDeviceptr_t base = nullptr;
+    size_t size = 0;
+    if (hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)ptr) != hipSuccess) {
+        (void)hipGetLastError(); // not every kind of memory has a range to ask for: nothing to compare with
+        return;
+    }
+    const uintptr_t end = (uintptr_t)base + size, p = (uintptr_t)ptr;
+    if (p < (uintptr_t)base || bytes > end - p)
+        fail(NBO_ERR_ARG, std::string(where) + ": " + std::to_string(bytes) + " bytes do not fit the allocation (" +
+                              std::to_string(end - p) + " bytes from there to its end)");
+}
+
 } // namespace nbo
 
 namespace {
@@ -338,41 +376,11 @@ uint32_t state_part_index(const nbo_optim *opt, char which)
     return which == 'm' ? 0 : opt->arena.part_v;
 }
 
-// A kernel that is handed a host address, or a shape larger than the allocation behind the
-// address, faults the GPU -- which can take the whole machine's GPUs down with it -- so every
-// tensor is checked against what the HIP runtime knows about its address before a list is
-// (re)bound: the address must be device-accessible memory the runtime has allocated or
-// registered, and the tensor must end inside that allocation.  (An allocator that hands out
-// pieces of a larger block is only checked against the block.)  NBO_CHECK_POINTERS=0 in the
-// environment skips the check.
-bool pointer_checks_enabled()
-{
-    static const bool on = [] {
-        const char *v = std::getenv("NBO_CHECK_POINTERS");
-        return !(v && v[0] == '0' && v[1] == '\0');
-    }();
-    return on;
-}
-
 void check_tensor_address(const void *ptr, uint64_t bytes, uint64_t t)
 {
-    char where[64];
-    std::snprintf(where, sizeof(where), "tensor %llu at %p", (unsigned long long)t, ptr);
-    hipPointerAttribute_t attr;
-    const hipError_t e = hipPointerGetAttributes(&attr, ptr);
-    if (e != hipSuccess) (void)hipGetLastError();
-    if (e != hipSuccess || attr.type == hipMemoryTypeUnregistered)
-        fail(NBO_ERR_ARG, std::string(where) + ": not memory the HIP runtime knows (a host pointer?)");
-    hipDeviceptr_t base = nullptr;
-    size_t size = 0;
-    if (hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)ptr) != hipSuccess) {
-        (void)hipGetLastError(); // not every kind of memory has a range to ask for: nothing to compare with
-        return;
-    }
-    const uintptr_t end = (uintptr_t)base + size, p = (uintptr_t)ptr;
-    if (p < (uintptr_t)base || bytes > end - p)
-        fail(NBO_ERR_ARG, std::string(where) + ": " + std::to_string(bytes) + " bytes do not fit the allocation (" +
-                              std::to_string(end - p) + " bytes from there to its end)");
+    char what[32];
+    std::snprintf(what, sizeof(what), "tensor %llu", (unsigned long long)t);
+    check_device_address(ptr, bytes, what);
 }
 
 // Copies the n elements of tensor i's part `part` between the arena and a dense

@@ -11,7 +11,8 @@
 
 // The gfx950 code object, embedded by nbo_code_object.S.
 extern "C" const unsigned char nbo_code_object[];
-// The measurement kernels' code object, likewise.
+// The operators' (include/nabla_ops.h) and the measurement kernels' code objects, likewise.
+extern "C" const unsigned char nbo_ops_code_object[];
 extern "C" const unsigned char nbo_bench_code_object[];
 
 namespace nbo {
@@ -60,10 +61,26 @@ static const char *const kKernelNames[K_COUNT] = {
     "nbo_update_f16_adamw_rows",   "nbo_update_f16_adam_rows",
     "nbo_accscale_f32",            "nbo_accscale_bf16",          "nbo_accscale_f64",
     "nbo_accscale_f16",            "nbo_selftest_bf16_arith",    "nbo_selftest_f16_arith",
+    "nbo_embed_f32",               "nbo_embed_bf16",             "nbo_embed_f64",
+    "nbo_embed_f16",               "nbo_embed_f32_bf16",         "nbo_embed_f32_f16",
+    "nbo_order_rank",              "nbo_order_hist",             "nbo_order_scan",
+    "nbo_order_scatter",
+    "nbo_embed_sum_f32",           "nbo_embed_sum_bf16",         "nbo_embed_sum_f64",
+    "nbo_embed_sum_f16",           "nbo_embed_sum_bf16_f32",     "nbo_embed_sum_f16_f32",
+    "nbo_embed_join_f32",          "nbo_embed_join_bf16",        "nbo_embed_join_f64",
+    "nbo_embed_join_f16",          "nbo_embed_join_bf16_f32",    "nbo_embed_join_f16_f32",
+    "nbo_embed_direct_f32",        "nbo_embed_direct_bf16",      "nbo_embed_direct_f64",
+    "nbo_embed_direct_f16",        "nbo_embed_direct_bf16_f32",  "nbo_embed_direct_f16_f32",
+    "nbo_dropout_f32",             "nbo_dropout_bf16",           "nbo_dropout_f64",
+    "nbo_dropout_f16",             "nbo_rng_advance",
 };
 static_assert(K_UPDATE_SELF_BASE + 18 == K_UPDATE_ROWS_BASE, "six families of three self-preparing update kernels");
-static_assert(K_UPDATE_ROWS_BASE + 8 == K_ACCSCALE_BASE && K_ACCSCALE_F16 + 3 == K_COUNT,
+static_assert(K_UPDATE_ROWS_BASE + 8 == K_ACCSCALE_BASE && K_ACCSCALE_F16 + 3 == K_OPS_BASE,
               "four families of two by-row update kernels, four micro-batch kernels without the sum");
+static_assert(K_EMBED_BASE == K_OPS_BASE && K_EMBED_BASE + 6 == K_ORDER_RANK && K_EMBED_SUM_BASE + 6 == K_EMBED_JOIN_BASE &&
+                  K_EMBED_JOIN_BASE + 6 == K_EMBED_DIRECT_BASE && K_EMBED_DIRECT_BASE + 6 == K_DROPOUT_BASE &&
+                  K_DROPOUT_BASE + 4 == K_RNG_ADVANCE && K_RNG_ADVANCE + 1 == K_COUNT,
+              "six element type pairs of each embedding kernel, four dropout kernels");
 
 static std::mutex g_runtime_mu;
 static Runtime *g_runtime = nullptr;
@@ -106,8 +123,11 @@ Runtime::Runtime()
              std::string("hipModuleLoadData of the embedded gfx950 code object failed: ") +
                  hipGetErrorString(e));
     }
+    hip_check(hipModuleLoadData(&ops_module_, nbo_ops_code_object), "hipModuleLoadData (operators)");
     for (int k = 0; k < K_COUNT; k++)
-        if (kKernelNames[k]) hip_check(hipModuleGetFunction(&fn_[k], module_, kKernelNames[k]), kKernelNames[k]);
+        if (kKernelNames[k])
+            hip_check(hipModuleGetFunction(&fn_[k], k < K_OPS_BASE ? module_ : ops_module_, kKernelNames[k]),
+                      kKernelNames[k]);
     pinned_bytes_ = 8 << 20; // two halves of 4 MiB
     hip_check(hipHostMalloc(&pinned_, pinned_bytes_, hipHostMallocDefault), "hipHostMalloc");
     for (hipEvent_t &e : staged_) hip_check(hipEventCreateWithFlags(&e, hipEventDisableTiming), "hipEventCreate");

@@ -13,6 +13,7 @@
 
 #include "../../../include/nabla_optim.h"
 #include "../nbo_device_types.h"
+#include "../nbo_ops_types.h"
 #include "nbo_placement.hpp"
 
 namespace nbo {
@@ -68,7 +69,19 @@ enum KernelId {
     K_ACCSCALE_F16 = 76,
     K_SELFTEST_BF16 = 77,
     K_SELFTEST_F16 = 78,
-    K_COUNT = 79 // ids from here on are measurement kernels, handed out by Runtime::bench_kernel
+    // the operators of nabla_ops.h, in a code object of their own
+    K_OPS_BASE = 79,
+    K_EMBED_BASE = 79,         // + pair: table and output f32, bf16, f64, f16, f32 -> bf16, f32 -> f16
+    K_ORDER_RANK = 85,
+    K_ORDER_HIST = 86,
+    K_ORDER_SCAN = 87,
+    K_ORDER_SCATTER = 88,
+    K_EMBED_SUM_BASE = 89,     // + pair: upstream gradient and gradient f32, bf16, f64, f16, bf16 -> f32, f16 -> f32
+    K_EMBED_JOIN_BASE = 95,    // + pair
+    K_EMBED_DIRECT_BASE = 101, // + pair
+    K_DROPOUT_BASE = 107,      // + element type (f32, bf16, f64, f16)
+    K_RNG_ADVANCE = 111,
+    K_COUNT = 112 // ids from here on are measurement kernels, handed out by Runtime::bench_kernel
 };
 
 // Lists of fewer chunks than this take the Adam kinds' by-row kernels (nbo_capi.cpp has the measurements).
@@ -153,6 +166,7 @@ private:
     hipFunction_t function(int kernel) const;
     const char *kernel_name(int kernel) const;
     hipModule_t module_ = nullptr;
+    hipModule_t ops_module_ = nullptr;
     hipFunction_t fn_[K_COUNT] = {};
     uint32_t grid_x_max_ = 0xFFFFFFu;
     hipModule_t bench_module_ = nullptr; // loaded on first use
@@ -224,12 +238,30 @@ struct nbo_optim {
     size_t elem_bytes() const { return state_dtype == NBO_DT_F64 ? 8 : nbo::is_half(state_dtype) ? 2 : 4; }
 };
 
+struct nbo_rng {
+    NboRngDev *dev = nullptr;
+};
+
+// Scratch of nbo_embedding_grad (nbo_ops.cpp has the sizes).
+struct nbo_embedding_ws {
+    uint64_t max_ids = 0, max_cols = 0;
+    uint32_t *keys[2] = {}, *pos[2] = {}; // the passes' source and destination
+    uint32_t *hist = nullptr, *totals = nullptr;
+    void *partial = nullptr;
+    uint64_t partial_bytes = 0;
+};
+
 // Buffers handed out by nbo_alloc_placed: whole arrays in named HBM regions.
 struct nbo_placed {
     nbo::StatePlacement placement;
 };
 
 namespace nbo {
+// Address checks (nbo_capi.cpp): whether they are on, and NBO_ERR_ARG unless `bytes` bytes at ptr lie in
+// memory the HIP runtime knows; `what` names the tensor in the message.
+bool pointer_checks_enabled();
+void check_device_address(const void *ptr, uint64_t bytes, const char *what);
+
 // NBLA tensor files (nbo_nbla.cpp)
 void nbla_save_list(const char *path, const nbo_list *list, const char *const *names);
 void nbla_load_list(const char *path, nbo_list *list, const char *const *names);

@@ -1,0 +1,105 @@
+// Plain-old-data argument blocks shared by the operator kernels (kernels/nbo_ops_kernels.hip) and
+// their host side (host/nbo_ops.cpp).  Element type codes are nbo_device_types.h's.
+#ifndef NBO_OPS_TYPES_H
+#define NBO_OPS_TYPES_H
+
+#include <stdint.h>
+
+#define NBO_OPS_BLOCK 256u // threads of every operator kernel but the ordering ones
+
+// The generator's state in device memory.
+struct NboRngDev {
+    uint64_t seed, step;
+};
+
+// Rows of `cols` elements cut into units of VEC elements (16 bytes of the 16-bit or wider type, see
+// Pair in the kernels), numbered through the matrix: row = unit / per_row.  m32 and m64 are
+// ceil(2^32 / per_row) and ceil(2^64 / per_row) (0 for per_row = 1).
+struct NboUnits {
+    uint64_t total;
+    uint64_t m64;
+    uint32_t per_row;
+    uint32_t m32;
+};
+
+struct NboEmbedArgs {
+    const void *table;
+    const void *ids;
+    const void *add; // may be null
+    void *out;
+    uint64_t table_stride, add_stride, out_stride; // bytes
+    NboUnits u;
+    double scale;
+    uint32_t rows, cols;
+    uint32_t ids64;
+    uint32_t pad;
+};
+
+struct NboDropoutArgs {
+    const void *x;
+    const void *residual; // may be null
+    void *out;
+    uint64_t x_stride, residual_stride, out_stride; // bytes
+    NboUnits u;
+    const NboRngDev *rng;
+    double scale;
+    uint64_t n;   // elements
+    uint32_t cols; // of a row of units; flat matrices are one row
+    uint32_t site;
+    uint32_t thr; // 0 .. 65536
+    uint32_t flat; // rows are adjacent: units run through the matrix
+};
+
+struct NboRngAdvanceArgs {
+    NboRngDev *rng;
+    uint64_t steps;
+};
+
+// ---- the gradient of the embedding ------------------------------------------------------
+// Keys: the ids, with every id outside the table replaced by `rows`, so that padding sorts last.
+
+// All-pairs ranking: one launch orders up to NBO_RANK_MAX ids.
+#define NBO_RANK_MAX 16384u
+#define NBO_RANK_BLOCK 1024u
+// Radix passes: ids per workgroup and the widest digit.
+#define NBO_RADIX_TILE 4096u
+#define NBO_RADIX_BLOCK 512u
+#define NBO_RADIX_BITS 10u
+// Up to this many ids the gradient is one launch that needs no order.
+#define NBO_EMBED_DIRECT_MAX 256u
+
+struct NboOrderArgs {
+    const void *ids;       // the caller's (first pass), or null: keys_in / pos_in
+    const uint32_t *keys_in, *pos_in;
+    uint32_t *keys_out, *pos_out;
+    uint32_t *hist;        // [digits][tiles]
+    uint32_t *totals;      // [digits]
+    uint32_t n;
+    uint32_t rows;
+    uint32_t ids64;
+    uint32_t tiles;
+    uint32_t shift, digits; // this pass's digit: (key >> shift) & (digits - 1)
+};
+
+struct NboEmbedGradArgs {
+    const void *dy;
+    void *grad;
+    const void *ids;              // the direct form only
+    const uint32_t *keys, *pos;   // in table order
+    void *partial;                // [pieces][2][units * VEC] sums of rows that span pieces
+    uint64_t dy_stride, grad_stride; // bytes
+    uint64_t row_bytes;           // of a row of grad
+    double scale;
+    uint32_t n, rows, cols;
+    uint32_t units;               // per row
+    uint32_t lanes;               // lanes that work on one piece: 64, or a power of two that holds `units`
+    uint32_t slabs;               // waves per piece (lanes == 64)
+    uint32_t piece, pieces;       // ids per piece, pieces
+    uint32_t sum_wgs, zero_wgs;   // workgroups that add, workgroups that clear rows no id names
+    uint32_t zero_rows;           // rows per clearing workgroup, at most 64
+    uint32_t accumulate;
+    uint32_t ids64;
+    uint32_t pad;
+};
+
+#endif
