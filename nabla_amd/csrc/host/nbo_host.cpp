@@ -63,8 +63,8 @@ static const char *const kKernelNames[K_COUNT] = {
     "nbo_accscale_f16",            "nbo_selftest_bf16_arith",    "nbo_selftest_f16_arith",
     "nbo_embed_f32",               "nbo_embed_bf16",             "nbo_embed_f64",
     "nbo_embed_f16",               "nbo_embed_f32_bf16",         "nbo_embed_f32_f16",
-    "nbo_order_rank",              "nbo_order_hist",             "nbo_order_scan",
-    "nbo_order_scatter",
+    "nbo_order_range",             "nbo_order_hist",             "nbo_order_scan",
+    "nbo_order_scatter",           "nbo_order_split",            "nbo_order_merge",
     "nbo_embed_sum_f32",           "nbo_embed_sum_bf16",         "nbo_embed_sum_f64",
     "nbo_embed_sum_f16",           "nbo_embed_sum_bf16_f32",     "nbo_embed_sum_f16_f32",
     "nbo_embed_join_f32",          "nbo_embed_join_bf16",        "nbo_embed_join_f64",
@@ -72,14 +72,14 @@ static const char *const kKernelNames[K_COUNT] = {
     "nbo_embed_direct_f32",        "nbo_embed_direct_bf16",      "nbo_embed_direct_f64",
     "nbo_embed_direct_f16",        "nbo_embed_direct_bf16_f32",  "nbo_embed_direct_f16_f32",
     "nbo_dropout_f32",             "nbo_dropout_bf16",           "nbo_dropout_f64",
-    "nbo_dropout_f16",             "nbo_rng_advance",
+    "nbo_dropout_f16",             "nbo_rng_advance",            "nbo_order_clear",
 };
 static_assert(K_UPDATE_SELF_BASE + 18 == K_UPDATE_ROWS_BASE, "six families of three self-preparing update kernels");
 static_assert(K_UPDATE_ROWS_BASE + 8 == K_ACCSCALE_BASE && K_ACCSCALE_F16 + 3 == K_OPS_BASE,
               "four families of two by-row update kernels, four micro-batch kernels without the sum");
-static_assert(K_EMBED_BASE == K_OPS_BASE && K_EMBED_BASE + 6 == K_ORDER_RANK && K_EMBED_SUM_BASE + 6 == K_EMBED_JOIN_BASE &&
+static_assert(K_EMBED_BASE == K_OPS_BASE && K_EMBED_BASE + 6 == K_ORDER_RANGE && K_EMBED_SUM_BASE + 6 == K_EMBED_JOIN_BASE &&
                   K_EMBED_JOIN_BASE + 6 == K_EMBED_DIRECT_BASE && K_EMBED_DIRECT_BASE + 6 == K_DROPOUT_BASE &&
-                  K_DROPOUT_BASE + 4 == K_RNG_ADVANCE && K_RNG_ADVANCE + 1 == K_COUNT,
+                  K_DROPOUT_BASE + 4 == K_RNG_ADVANCE && K_RNG_ADVANCE + 2 == K_COUNT,
               "six element type pairs of each embedding kernel, four dropout kernels");
 
 static std::mutex g_runtime_mu;

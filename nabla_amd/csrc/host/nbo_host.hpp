@@ -72,16 +72,19 @@ enum KernelId {
     // the operators of nabla_ops.h, in a code object of their own
     K_OPS_BASE = 79,
     K_EMBED_BASE = 79,         // + pair: table and output f32, bf16, f64, f16, f32 -> bf16, f32 -> f16
-    K_ORDER_RANK = 85,
+    K_ORDER_RANGE = 85,
     K_ORDER_HIST = 86,
     K_ORDER_SCAN = 87,
     K_ORDER_SCATTER = 88,
-    K_EMBED_SUM_BASE = 89,     // + pair: upstream gradient and gradient f32, bf16, f64, f16, bf16 -> f32, f16 -> f32
-    K_EMBED_JOIN_BASE = 95,    // + pair
-    K_EMBED_DIRECT_BASE = 101, // + pair
-    K_DROPOUT_BASE = 107,      // + element type (f32, bf16, f64, f16)
-    K_RNG_ADVANCE = 111,
-    K_COUNT = 112 // ids from here on are measurement kernels, handed out by Runtime::bench_kernel
+    K_ORDER_SPLIT = 89,
+    K_ORDER_MERGE = 90,
+    K_EMBED_SUM_BASE = 91,     // + pair: upstream gradient and gradient f32, bf16, f64, f16, bf16 -> f32, f16 -> f32
+    K_EMBED_JOIN_BASE = 97,    // + pair
+    K_EMBED_DIRECT_BASE = 103, // + pair
+    K_DROPOUT_BASE = 109,      // + element type (f32, bf16, f64, f16)
+    K_RNG_ADVANCE = 113,
+    K_ORDER_CLEAR = 114,
+    K_COUNT = 115 // ids from here on are measurement kernels, handed out by Runtime::bench_kernel
 };
 
 // Lists of fewer chunks than this take the Adam kinds' by-row kernels (nbo_capi.cpp has the measurements).
@@ -242,11 +245,13 @@ struct nbo_rng {
     NboRngDev *dev = nullptr;
 };
 
-// Scratch of nbo_embedding_grad (nbo_ops.cpp has the sizes).
+// Scratch of nbo_embedding_grad (nbo_ops.cpp has the sizes): pieces of one allocation.
 struct nbo_embedding_ws {
     uint64_t max_ids = 0, max_cols = 0;
+    void *blob = nullptr;
     uint32_t *keys[2] = {}, *pos[2] = {}; // the passes' source and destination
     uint32_t *hist = nullptr, *totals = nullptr;
+    uint8_t *named = nullptr;
     void *partial = nullptr;
     uint64_t partial_bytes = 0;
 };

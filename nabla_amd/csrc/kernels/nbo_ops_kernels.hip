@@ -2,9 +2,11 @@
 // and dropout from a counter-based generator.  A code object of its own beside the optimizer's.
 //
 //   nbo_embed_*        out[t] = add[t] + scale * table[ids[t]]
-//   nbo_order_rank     the ids in table order, by comparing all pairs (few ids)
-//   nbo_order_hist / _scan / _scatter   ... by radix passes (many ids)
-//   nbo_embed_sum_*    grad[v] (+)= scale * sum of the rows of dy that name v, in pieces of the order
+//   nbo_order_range    the ids in table order, in one launch (up to some 10^5 ids)
+//   nbo_order_split / _merge   ... in two (more ids), nbo_order_hist / _scan / _scatter   ... by radix passes (more rows)
+//   nbo_order_clear    zeros in the rows no id names, behind the radix passes
+//   nbo_embed_sum_*    grad[v] (+)= scale * sum of the rows of dy that name v, in pieces of the order; zeros in the
+//                      rows no id names
 //   nbo_embed_join_*   ... of the rows whose tokens span pieces
 //   nbo_embed_direct_* the whole gradient in one launch, for a few ids
 //   nbo_dropout_*      out = residual + kept(x) * scale
@@ -65,6 +67,9 @@ template <> struct El<NBO_F16> {
     DEV Bits narrow(A x) { return __builtin_bit_cast(Bits, (_Float16)x); }
 };
 
+// Loads that are to be in flight together stand outside of branches (what a lane must not use is loaded
+// from a place that exists): at the end of a branch that loads, the compiler may wait.
+
 // A unit of V elements of type E as it lies in memory: 16 bytes, or 32 where the other tensor of the
 // operator has elements of half the size.
 template <int E, int V> struct Unit {
@@ -72,11 +77,14 @@ template <int E, int V> struct Unit {
     typedef typename El<E>::A A;
     enum { SZ = sizeof(Bits), PER = 16 / SZ, N = V * SZ / 16 };
     u32x4 w[N];
-    __device__ __forceinline__ void load(const char *p, uint32_t n) // n < V: a matrix narrower than a unit
+    // TINY: the matrix is narrower than a unit, n < V.  ONCE: the bytes are not needed again soon
+    template <bool TINY, bool ONCE> __device__ __forceinline__ void load(const char *p, uint32_t n)
     {
-        if (n == V) {
+        if (!TINY) {
 #pragma unroll
-            for (int k = 0; k < N; k++) w[k] = *GLOBAL_PTR(const u32x4_e, p + 16 * k);
+            for (int k = 0; k < N; k++)
+                w[k] = ONCE ? __builtin_nontemporal_load(GLOBAL_PTR(const u32x4_e, p + 16 * k))
+                            : *GLOBAL_PTR(const u32x4_e, p + 16 * k);
         } else {
             A x[V];
 #pragma unroll
@@ -109,11 +117,14 @@ template <int E, int V> struct Unit {
         }
     }
     // elements skip .. n - 1
-    __device__ __forceinline__ void store(char *p, uint32_t skip, uint32_t n) const
+    template <bool ONCE> __device__ __forceinline__ void store(char *p, uint32_t skip, uint32_t n) const
     {
         if (skip == 0 && n == V) {
 #pragma unroll
-            for (int k = 0; k < N; k++) *GLOBAL_PTR(u32x4_e, p + 16 * k) = w[k];
+            for (int k = 0; k < N; k++) {
+                if (ONCE) __builtin_nontemporal_store((u32x4_e)w[k], GLOBAL_PTR(u32x4_e, p + 16 * k));
+                else *GLOBAL_PTR(u32x4_e, p + 16 * k) = w[k];
+            }
             return;
         }
 #pragma unroll
@@ -187,17 +198,27 @@ DEV void unit_at(const NboUnits &u, const UnitBase &b, uint32_t x, uint64_t *row
 // the id of token t as a row of the table, or `rows` for an id outside it
 DEV uint32_t load_key(const void *ids, uint32_t ids64, uint64_t t, uint32_t rows)
 {
+    const uint64_t id = ids64 ? GLOBAL_PTR(const uint64_t, ids)[t] : (uint64_t)GLOBAL_PTR(const uint32_t, ids)[t];
+    return id < rows ? (uint32_t)id : rows;
+}
+// ... of U tokens at once: a branch that used what it loads would wait for it, so the keys come after all loads
+template <int U> DEV void load_keys(const void *ids, uint32_t ids64, const uint64_t (&t)[U], uint32_t rows, uint32_t (&key)[U])
+{
+    uint64_t id[U];
     if (ids64) {
-        const uint64_t id = GLOBAL_PTR(const uint64_t, ids)[t];
-        return id < rows ? (uint32_t)id : rows;
+#pragma unroll
+        for (int k = 0; k < U; k++) id[k] = GLOBAL_PTR(const uint64_t, ids)[t[k]];
+    } else {
+#pragma unroll
+        for (int k = 0; k < U; k++) id[k] = GLOBAL_PTR(const uint32_t, ids)[t[k]];
     }
-    const uint32_t id = GLOBAL_PTR(const uint32_t, ids)[t];
-    return id < rows ? id : rows;
+#pragma unroll
+    for (int k = 0; k < U; k++) key[k] = id[k] < rows ? (uint32_t)id[k] : rows;
 }
 
 // ---------------------------------------------------------------------------------
 // The lookup: U units per thread, all ids read, then all rows, then all stores.
-template <int ET, int EO, int U> DEV void embed_body(const NboEmbedArgs &a)
+template <int ET, int EO, int U, bool TINY> DEV void embed_body(const NboEmbedArgs &a)
 {
     enum { V = Pair<ET, EO>::V, ST = sizeof(typename El<ET>::Bits), SO = sizeof(typename El<EO>::Bits) };
     typedef typename El<EO>::A A;
@@ -211,17 +232,29 @@ template <int ET, int EO, int U> DEV void embed_body(const NboEmbedArgs &a)
     for (int k = 0; k < U; k++) {
         const uint32_t x = threadIdx.x + k * NBO_OPS_BLOCK;
         on[k] = base + x < a.u.total;
-        unit_at(a.u, b, x, &t[k], &v[k]);
-        key[k] = on[k] ? load_key(a.ids, a.ids64, t[k], a.rows) : a.rows;
+        // (what is beyond the end looks at the first unit again and stores nothing)
+        unit_at(a.u, b, on[k] ? x : 0, &t[k], &v[k]);
     }
+    load_keys<U>(a.ids, a.ids64, t, a.rows, key);
     Unit<ET, V> row[U];
     Unit<EO, V> add[U];
+    if (a.rows > 0) {
 #pragma unroll
-    for (int k = 0; k < U; k++) {
-        const Span s = unit_span<V>(v[k], a.cols);
-        row[k].clear();
-        if (key[k] < a.rows) row[k].load((const char *)a.table + key[k] * a.table_stride + (uint64_t)s.c0 * ST, s.n);
-        if (a.add && on[k]) add[k].load((const char *)a.add + t[k] * a.add_stride + (uint64_t)s.c0 * SO, s.n);
+        for (int k = 0; k < U; k++) { // (padding looks at row 0)
+            const Span s = unit_span<V>(v[k], a.cols);
+            const uint64_t r = key[k] < a.rows ? key[k] : 0;
+            row[k].template load<TINY, false>((const char *)a.table + r * a.table_stride + (uint64_t)s.c0 * ST, s.n);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < U; k++) row[k].clear();
+    }
+    if (a.add) {
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            const Span s = unit_span<V>(v[k], a.cols);
+            add[k].template load<TINY, false>((const char *)a.add + t[k] * a.add_stride + (uint64_t)s.c0 * SO, s.n);
+        }
     }
     const A scale = (A)a.scale;
 #pragma unroll
@@ -241,14 +274,15 @@ template <int ET, int EO, int U> DEV void embed_body(const NboEmbedArgs &a)
         }
         Unit<EO, V> o;
         o.pack(x);
-        o.store((char *)a.out + t[k] * a.out_stride + (uint64_t)s.c0 * SO, s.skip, s.n);
+        o.template store<true>((char *)a.out + t[k] * a.out_stride + (uint64_t)s.c0 * SO, s.skip, s.n);
     }
 }
 
 #define NBO_EMBED_KERNEL(name, ET, EO)                                                      \
     extern "C" __global__ __launch_bounds__(NBO_OPS_BLOCK) void name(const NboEmbedArgs a)  \
     {                                                                                       \
-        embed_body<ET, EO, 1>(a);                                                           \
+        if (a.cols >= (uint32_t)Pair<ET, EO>::V) embed_body<ET, EO, NBO_EMBED_UNITS, false>(a); \
+        else embed_body<ET, EO, NBO_EMBED_UNITS, true>(a);                                  \
     }
 NBO_EMBED_KERNEL(nbo_embed_f32, NBO_F32, NBO_F32)
 NBO_EMBED_KERNEL(nbo_embed_bf16, NBO_BF16, NBO_BF16)
@@ -257,52 +291,188 @@ NBO_EMBED_KERNEL(nbo_embed_f16, NBO_F16, NBO_F16)
 NBO_EMBED_KERNEL(nbo_embed_f32_bf16, NBO_F32, NBO_BF16)
 NBO_EMBED_KERNEL(nbo_embed_f32_f16, NBO_F32, NBO_F16)
 
-// ---------------------------------------------------------------------------------
-// Table order by all pairs: a token's place is the number of (key, token) pairs before its own.
-// One workgroup ranks 64 tokens, one per lane; its sixteen waves share the ids, which lie in LDS.
-extern "C" __global__ __launch_bounds__(NBO_RANK_BLOCK) void nbo_order_rank(const NboOrderArgs a)
+// inclusive sum over the wave
+DEV uint32_t wave_scan(uint32_t x)
 {
-    enum { WAVES = NBO_RANK_BLOCK / 64 };
-    __shared__ uint32_t keys[NBO_RANK_MAX];
-    __shared__ uint32_t before[WAVES][64];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t blocks = (a.n + 63) / 64; // of 64 keys; the last is filled up with keys that are before none
-    for (uint32_t i = threadIdx.x; i < blocks * 64; i += NBO_RANK_BLOCK)
-        keys[i] = i < a.n ? load_key(a.ids, a.ids64, i, a.rows) : 0xFFFFFFFFu;
-    __syncthreads();
-    const uint32_t own = blockIdx.x, mine = keys[own * 64 + lane];
-    const uint32_t per = (blocks + WAVES - 1) / WAVES;
-    const uint32_t lo = wave * per, hi = lo + per < blocks ? lo + per : blocks;
-    uint32_t cnt = 0;
-    for (uint32_t blk = lo; blk < hi; blk++) {
-        const u32x4 *k4 = (const u32x4 *)(keys + blk * 64);
-        if (blk == own) {
-            for (uint32_t j = 0; j < 64; j++) {
-                const uint32_t k = keys[blk * 64 + j];
-                cnt += k < mine || (k == mine && j < lane);
-            }
-        } else {
-            // equal keys of earlier blocks are before this one's, of later blocks behind
-            const uint32_t bound = blk < own ? mine + 1 : mine;
-#pragma unroll 4
-            for (uint32_t j = 0; j < 16; j++) {
-                const u32x4 k = k4[j];
-                cnt += k.x < bound;
-                cnt += k.y < bound;
-                cnt += k.z < bound;
-                cnt += k.w < bound;
-            }
-        }
-    }
-    before[wave][lane] = cnt;
-    __syncthreads();
-    const uint32_t t = own * 64 + lane;
-    if (wave == 0 && t < a.n) {
-        uint32_t rank = 0;
+    const uint32_t lane = threadIdx.x & 63u;
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) rank += before[w][lane];
-        GLOBAL_PTR(uint32_t, a.keys_out)[rank] = mine;
-        GLOBAL_PTR(uint32_t, a.pos_out)[rank] = t;
+    for (int s = 1; s < 64; s *= 2) {
+        const uint32_t y = __shfl_up(x, s);
+        if (lane >= (uint32_t)s) x += y;
+    }
+    return x;
+}
+
+// ---------------------------------------------------------------------------------
+// Table order in one launch: every workgroup owns a range of keys, reads all ids and puts those of its
+// range to their places.  Nothing passes between workgroups: how many ids come before the range is
+// counted on the way.  Within the range an id's place is its key's start, the ids of that key which
+// earlier waves hold (each wave has a run of the ids), and those its own wave has seen.
+
+// For a block of 64 ids of which the lanes in `left` (not empty) count: adds to mine[r] how many lanes hold
+// each r.  The lanes that hold what the first one holds are counted as one: an addition to one LDS word takes
+// a turn for every lane, and a hot row fills whole blocks.
+DEV void count_keys(uint32_t *mine, uint32_t r, uint64_t left)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    const int first = __builtin_ctzll(left);
+    const uint64_t m = left & __builtin_amdgcn_ballot_w64(r == (uint32_t)__builtin_amdgcn_readlane(r, first));
+    if ((int)lane == first) atomicAdd(&mine[r], (uint32_t)__popcll(m));
+    if ((left & ~m) >> lane & 1) atomicAdd(&mine[r], 1u);
+}
+
+DEV uint32_t lanes_before(uint64_t m)
+{
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+
+// ... and with mine[r] the place of the next id that has r (r < 2^bits): each lane's place, in the order of
+// the lanes.  The counters are one wave's own, so nothing else moves them.  First the lanes that hold what
+// the first one holds (all of them, where a row is hot); one or two more one by one; more than that
+// together: who holds the same r is found bit by bit.
+DEV uint32_t place_keys(uint32_t *mine, uint32_t r, uint64_t left, uint32_t bits)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    const int first = __builtin_ctzll(left);
+    uint64_t same = left & __builtin_amdgcn_ballot_w64(r == (uint32_t)__builtin_amdgcn_readlane(r, first));
+    uint32_t at = 0;
+    if ((int)lane == first) at = atomicAdd(&mine[r], (uint32_t)__popcll(same));
+    const uint32_t next = __builtin_amdgcn_readlane(at, first);
+    if (same >> lane & 1) at = next + lanes_before(same);
+    left &= ~same;
+    if (__popcll(left) <= 2) {
+        for (; left; left &= left - 1)
+            if ((int)lane == __builtin_ctzll(left)) at = atomicAdd(&mine[r], 1u);
+        return at;
+    }
+    const bool on = left >> lane & 1;
+    same = left;
+    for (uint32_t b = 0; b < bits; b++) {
+        const uint64_t m = __builtin_amdgcn_ballot_w64((r >> b & 1) != 0);
+        same &= (r >> b & 1) ? m : ~m;
+    }
+    const uint32_t ahead = lanes_before(same);
+    uint32_t start = 0;
+    if (on && ahead == 0) start = atomicAdd(&mine[r], (uint32_t)__popcll(same));
+    start = __shfl(start, on ? __builtin_ctzll(same) : 0);
+    return on ? start + ahead : at;
+}
+
+// count[WAVES][range], each wave's number of ids of each key, becomes where the wave's first one goes:
+// behind the `below` (summed over the waves) ids before the range, the smaller keys, the waves before.
+// One thread per key; range is at most the workgroup's size.  Notes in a.named which rows of the table have
+// ids (lo: the range's first key).
+template <int WAVES> DEV void starts_of_keys(const NboOrderArgs &a, uint32_t lo, uint32_t *count, uint32_t range,
+                                             uint32_t below, uint32_t (&wsum)[WAVES], uint32_t (&wbelow)[WAVES])
+{
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int s = 32; s >= 1; s /= 2) below += __shfl_xor(below, s);
+    if (lane == 0) wbelow[wave] = below;
+    __syncthreads();
+    uint32_t c[WAVES], total = 0;
+    if (threadIdx.x < range)
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) total += c[w] = count[w * range + threadIdx.x];
+    if (a.named && threadIdx.x < range && lo + threadIdx.x < a.rows)
+        GLOBAL_PTR(uint8_t, a.named)[lo + threadIdx.x] = total > 0;
+    const uint32_t up = wave_scan(total);
+    if (lane == 63) wsum[wave] = up;
+    __syncthreads();
+    uint32_t at = up - total;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        at += wbelow[w];
+        if ((uint32_t)w < wave) at += wsum[w];
+    }
+    if (threadIdx.x < range)
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            count[w * range + threadIdx.x] = at;
+            at += c[w];
+        }
+    __syncthreads();
+}
+
+template <int U> DEV void range_keys(const NboOrderArgs &a, uint32_t blk, uint32_t (&key)[U])
+{
+    uint64_t t[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) { // (behind the last id: that one again)
+        const uint64_t i = (uint64_t)(blk + u) * 64 + (threadIdx.x & 63u);
+        t[u] = i < a.n ? i : a.n - 1;
+    }
+    load_keys<U>(a.ids, a.ids64, t, a.rows, key);
+}
+
+// Zeros in `bytes` bytes (an even number) at an even address, by a whole wave: two bytes at a time up to
+// the first 16-byte boundary and behind the last.
+DEV void clear_bytes(char *p, uint64_t bytes)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint64_t to_boundary = (16u - (uint32_t)((uintptr_t)p & 15u)) & 15u;
+    const uint64_t head = to_boundary < bytes ? to_boundary : bytes, nvec = (bytes - head) / 16, tail = head + nvec * 16;
+    const u32x4 z = 0;
+    char *v = p + head;
+#pragma unroll 4
+    for (uint64_t i = lane; i < nvec; i += 64) __builtin_nontemporal_store(z, GLOBAL_PTR(u32x4, v + i * 16));
+    if (lane * 2 < head) *GLOBAL_PTR(uint16_t, p + lane * 2) = 0;
+    if (lane * 2 < bytes - tail) *GLOBAL_PTR(uint16_t, p + tail + lane * 2) = 0;
+}
+
+// Zeros in the rows first .. first + count - 1 (count <= 64) whose bit in `named` is not set.  Rows that are
+// adjacent in memory are cleared as one run.
+DEV void clear_rows(const NboClearArgs &c, uint64_t first, uint32_t count, uint64_t named)
+{
+    uint64_t left = ~named & (count < 64 ? (1ull << count) - 1 : ~0ull);
+    while (left) {
+        const uint32_t r = __builtin_ctzll(left);
+        const uint64_t run = ~(left >> r); // bit k: row r + k is not to be cleared
+        uint32_t k = c.grad_stride == c.row_bytes ? (run ? (uint32_t)__builtin_ctzll(run) : 64u) : 1u;
+        clear_bytes((char *)c.grad + (first + r) * c.grad_stride, k * c.row_bytes);
+        left = r + k < 64 ? left >> (r + k) << (r + k) : 0;
+    }
+}
+
+extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_range(const NboOrderArgs a)
+{
+    enum { WAVES = NBO_RANGE_BLOCK / 64, U = NBO_RANGE_IDS / NBO_RANGE_BLOCK };
+    extern __shared__ uint32_t count[]; // [WAVES][range]
+    __shared__ uint32_t wsum[WAVES], wbelow[WAVES];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t blocks = (a.n + 63) / 64, per = (blocks + WAVES - 1) / WAVES; // blocks of 64 ids per wave, at most U
+    const uint32_t lo = blockIdx.x * a.range, first = wave * per * 64 + lane;
+    uint64_t t[U];
+    uint32_t key[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) { // (behind the wave's or the last id: that one again)
+        const uint32_t i = first + ((uint32_t)u < per ? u : per - 1) * 64;
+        t[u] = i < a.n ? i : a.n - 1;
+    }
+    load_keys<U>(a.ids, a.ids64, t, a.rows, key);
+    for (uint32_t i = threadIdx.x; i < WAVES * a.range; i += NBO_RANGE_BLOCK) count[i] = 0;
+    __syncthreads();
+    uint32_t *mine = count + wave * a.range;
+    uint32_t below = 0;
+    uint64_t in[U]; // the lanes whose ids are in the range
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const bool on = (uint32_t)u < per && first + u * 64 < a.n;
+        below += on && key[u] < lo;
+        key[u] -= lo;
+        in[u] = __builtin_amdgcn_ballot_w64(on && key[u] < a.range);
+        if (in[u]) count_keys(mine, key[u], in[u]);
+    }
+    starts_of_keys<WAVES>(a, lo, count, a.range, below, wsum, wbelow);
+    const uint32_t bits = 32 - __builtin_clz(a.range | 1);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (!in[u]) continue;
+        const uint32_t at = place_keys(mine, key[u], in[u], bits);
+        if (in[u] >> lane & 1) {
+            GLOBAL_PTR(uint32_t, a.keys_out)[at] = key[u] + lo;
+            GLOBAL_PTR(uint32_t, a.pos_out)[at] = first + u * 64;
+        }
     }
 }
 
@@ -331,18 +501,6 @@ extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_hist(con
         GLOBAL_PTR(uint32_t, a.hist)[(uint64_t)d * a.tiles + blockIdx.x] = count[d];
 }
 
-// inclusive sum over the wave
-DEV uint32_t wave_scan(uint32_t x)
-{
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) {
-        const uint32_t y = __shfl_up(x, s);
-        if (lane >= (uint32_t)s) x += y;
-    }
-    return x;
-}
-
 // one wave per digit
 extern "C" __global__ __launch_bounds__(64) void nbo_order_scan(const NboOrderArgs a)
 {
@@ -358,6 +516,36 @@ extern "C" __global__ __launch_bounds__(64) void nbo_order_scan(const NboOrderAr
     if (threadIdx.x == 0) GLOBAL_PTR(uint32_t, a.totals)[blockIdx.x] = sum;
 }
 
+// For the ROWS rows of 64 ids that a wave takes in order, with digits d: how many ids of its digit come
+// before each in the wave, and in mine[digit] how many there are.
+template <int ROWS> DEV void rank_digits(uint32_t *mine, const uint32_t (&d)[ROWS], const bool (&on)[ROWS], uint32_t digits,
+                                         uint32_t (&rank)[ROWS])
+{
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+        uint64_t same = __builtin_amdgcn_ballot_w64(on[r]);
+        for (uint32_t bit = 1; bit < digits; bit <<= 1) { // lanes with the same digit
+            const uint64_t m = __builtin_amdgcn_ballot_w64((d[r] & bit) != 0);
+            same &= (d[r] & bit) ? m : ~m;
+        }
+        const uint32_t ahead = lanes_before(same);
+        uint32_t seen = 0;
+        if (on[r] && ahead == 0) seen = atomicAdd(&mine[d[r]], (uint32_t)__popcll(same)); // (the wave's own counter)
+        rank[r] = __shfl(seen, on[r] ? __builtin_ctzll(same) : 0) + ahead;
+    }
+}
+
+// exclusive sums over a workgroup of NBO_RADIX_BLOCK threads
+DEV uint32_t block_starts(uint32_t x, uint32_t (&wsum)[NBO_RADIX_BLOCK / 64])
+{
+    const uint32_t wave = threadIdx.x >> 6, up = wave_scan(x);
+    if ((threadIdx.x & 63u) == 63) wsum[wave] = up;
+    __syncthreads();
+    uint32_t below = up - x;
+    for (uint32_t w = 0; w < wave; w++) below += wsum[w];
+    return below;
+}
+
 extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_scatter(const NboOrderArgs a)
 {
     enum { WAVES = NBO_RADIX_BLOCK / 64, ROWS = NBO_RADIX_TILE / NBO_RADIX_BLOCK };
@@ -367,36 +555,19 @@ extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_scatter(
     for (uint32_t d = threadIdx.x; d < a.digits; d += NBO_RADIX_BLOCK)
 #pragma unroll
         for (int w = 0; w < WAVES; w++) count[w][d] = 0;
-    // each wave takes a run of the tile, in order, 64 ids at a time
     const uint32_t first = blockIdx.x * NBO_RADIX_TILE + wave * (ROWS * 64) + lane;
-    uint32_t key[ROWS], pos[ROWS], rank[ROWS];
+    uint32_t key[ROWS], pos[ROWS], rank[ROWS], digit[ROWS];
+    bool on[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; r++) {
         const uint32_t i = first + r * 64;
-        key[r] = i < a.n ? order_key(a, i) : 0;
-        pos[r] = i < a.n ? (a.pos_in ? GLOBAL_PTR(const uint32_t, a.pos_in)[i] : i) : 0;
+        on[r] = i < a.n;
+        key[r] = on[r] ? order_key(a, i) : 0;
+        pos[r] = on[r] ? (a.pos_in ? GLOBAL_PTR(const uint32_t, a.pos_in)[i] : i) : 0;
+        digit[r] = (key[r] >> a.shift) & (a.digits - 1);
     }
     __syncthreads();
-    volatile uint32_t *mine = count[wave];
-#pragma unroll
-    for (int r = 0; r < ROWS; r++) {
-        const bool on = first + r * 64 < a.n;
-        const uint32_t d = (key[r] >> a.shift) & (a.digits - 1);
-        uint64_t same = __builtin_amdgcn_ballot_w64(on);
-        for (uint32_t bit = 1; bit < a.digits; bit <<= 1) { // lanes with the same digit
-            const uint64_t m = __builtin_amdgcn_ballot_w64((d & bit) != 0);
-            same &= (d & bit) ? m : ~m;
-        }
-        const uint32_t ahead = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
-        uint32_t seen = 0;
-        if (on) seen = mine[d];
-        rank[r] = seen + ahead;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (on && ahead == 0) mine[d] = seen + (uint32_t)__popcll(same);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    }
+    rank_digits<ROWS>(count[wave], digit, on, a.digits, rank);
     __syncthreads();
     // where each digit starts: the digits below it, the tiles before this one, the waves before each
     const uint32_t per = (a.digits + NBO_RADIX_BLOCK - 1) / NBO_RADIX_BLOCK; // at most 2
@@ -405,11 +576,7 @@ extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_scatter(
         const uint32_t d = threadIdx.x * per + k;
         if (d < a.digits) tot[k] = GLOBAL_PTR(const uint32_t, a.totals)[d];
     }
-    const uint32_t up = wave_scan(tot[0] + tot[1]);
-    if (lane == 63) wsum[wave] = up;
-    __syncthreads();
-    uint32_t below = up - (tot[0] + tot[1]);
-    for (uint32_t w = 0; w < wave; w++) below += wsum[w];
+    uint32_t below = block_starts(tot[0] + tot[1], wsum);
     for (uint32_t k = 0; k < per; k++) {
         const uint32_t d = threadIdx.x * per + k;
         if (d >= a.digits) break;
@@ -425,63 +592,156 @@ extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_scatter(
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < ROWS; r++)
-        if (first + r * 64 < a.n) {
-            const uint32_t at = count[wave][(key[r] >> a.shift) & (a.digits - 1)] + rank[r];
+        if (on[r]) {
+            const uint32_t at = count[wave][digit[r]] + rank[r];
             GLOBAL_PTR(uint32_t, a.keys_out)[at] = key[r];
             GLOBAL_PTR(uint32_t, a.pos_out)[at] = pos[r];
         }
 }
 
 // ---------------------------------------------------------------------------------
-// The sums.  The order is cut into pieces of a.piece tokens; `lanes` lanes, one unit of the row each,
-// walk a piece and add up the rows of dy.  A row of the table all of whose tokens lie in the piece is
-// finished there; the sums of one that began in an earlier piece or goes on into the next are left in
-// the piece's two slots, for the join.  So a row that half the batch names is added up by many
-// waves, and in the same order of additions on every run.
-template <int EG, int V> DEV void add_to_grad(const NboEmbedGradArgs &a, uint32_t key, const Span &s,
-                                              typename El<EG>::A (&x)[V])
+// Table order in two launches: every tile puts its ids in the order of the keys' high bits, in place,
+// and notes where each of these ranges starts; then one workgroup per range collects it from all tiles
+// and orders it as nbo_order_range does.  What lies before the range is the sum of the tiles' starts.
+extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_split(const NboOrderArgs a)
 {
-    typedef typename El<EG>::A A;
-    char *p = (char *)a.grad + key * a.grad_stride + (uint64_t)s.c0 * sizeof(typename El<EG>::Bits);
-    const A scale = (A)a.scale;
-    Unit<EG, V> g;
-    if (a.accumulate) {
-        A y[V];
-        g.load(p, s.n);
-        g.unpack(y);
+    enum { WAVES = NBO_RADIX_BLOCK / 64, ROWS = NBO_SPLIT_TILE / NBO_RADIX_BLOCK };
+    __shared__ uint32_t count[WAVES][1u << NBO_RADIX_BITS];
+    __shared__ uint32_t wsum[WAVES];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    for (uint32_t d = threadIdx.x; d < a.digits; d += NBO_RADIX_BLOCK)
 #pragma unroll
-        for (int j = 0; j < V; j++) x[j] = y[j] + scale * x[j];
-    } else {
+        for (int w = 0; w < WAVES; w++) count[w][d] = 0;
+    const uint32_t tile = blockIdx.x * NBO_SPLIT_TILE, first = tile + wave * (ROWS * 64) + lane;
+    uint32_t key[ROWS], rank[ROWS], digit[ROWS];
+    uint64_t t[ROWS];
+    bool on[ROWS];
 #pragma unroll
-        for (int j = 0; j < V; j++) x[j] = scale * x[j];
+    for (int r = 0; r < ROWS; r++) {
+        on[r] = first + r * 64 < a.n;
+        t[r] = on[r] ? first + r * 64 : a.n - 1;
     }
-    g.pack(x);
-    g.store(p, s.skip, s.n);
+    load_keys<ROWS>(a.ids, a.ids64, t, a.rows, key);
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) digit[r] = key[r] >> a.shift;
+    __syncthreads();
+    rank_digits<ROWS>(count[wave], digit, on, a.digits, rank);
+    __syncthreads();
+    uint32_t tot[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t d = threadIdx.x * 2 + k;
+        if (d < a.digits)
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) tot[k] += count[w][d];
+    }
+    uint32_t at = block_starts(tot[0] + tot[1], wsum);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t d = threadIdx.x * 2 + k;
+        if (d >= a.digits) break;
+        GLOBAL_PTR(uint32_t, a.hist)[(uint64_t)d * a.tiles + blockIdx.x] = at;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const uint32_t c = count[w][d];
+            count[w][d] = at;
+            at += c;
+        }
+    }
+    if (threadIdx.x == 0) // where a range behind the last one would start
+        GLOBAL_PTR(uint32_t, a.hist)[(uint64_t)a.digits * a.tiles + blockIdx.x] =
+            a.n - tile < NBO_SPLIT_TILE ? a.n - tile : NBO_SPLIT_TILE;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROWS; r++)
+        if (on[r]) {
+            const uint32_t i = tile + count[wave][digit[r]] + rank[r];
+            GLOBAL_PTR(uint32_t, a.keys_out)[i] = key[r];
+            GLOBAL_PTR(uint32_t, a.pos_out)[i] = first + r * 64;
+        }
 }
 
-enum { SLOT_HEAD = 0, SLOT_TAIL = 1 }; // began in an earlier piece / goes on into the next only
-template <typename A, int V> DEV char *slot_at(const NboEmbedGradArgs &a, uint32_t piece, uint32_t slot, uint32_t v)
+extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(const NboOrderArgs a)
 {
-    return (char *)a.partial + (((uint64_t)piece * 2 + slot) * a.units + v) * (V * sizeof(A));
-}
-template <typename A, int V> DEV void store_slot(char *p, const A (&x)[V])
-{
+    enum { WAVES = NBO_RANGE_BLOCK / 64, U = 4 };
+    __shared__ uint32_t count[WAVES << NBO_SPLIT_SHIFT];
+    __shared__ uint32_t wsum[WAVES], wbelow[WAVES];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
+    const uint32_t range = 1u << a.shift, lo = blockIdx.x << a.shift;
+    auto *h = GLOBAL_PTR(const uint32_t, a.hist) + (uint64_t)blockIdx.x * a.tiles;
+    auto *keys = GLOBAL_PTR(const uint32_t, a.keys_in);
+    auto *poss = GLOBAL_PTR(const uint32_t, a.pos_in);
+    const uint32_t per = (a.tiles + WAVES - 1) / WAVES;
+    const uint32_t from = wave * per, to = from + per < a.tiles ? from + per : a.tiles;
+    uint32_t below = 0;
+    for (uint32_t t = threadIdx.x; t < a.tiles; t += NBO_RANGE_BLOCK) below += h[t];
+    for (uint32_t i = threadIdx.x; i < WAVES * range; i += NBO_RANGE_BLOCK) count[i] = 0;
+    uint32_t *mine = count + wave * range;
+    // The wave's tiles in order, four at a time: the first 64 ids of the range in each of the four are asked
+    // for together, with their places, and kept where there is but one such group (up to 64 tiles)
+    uint32_t at[U], len[U], key[U], pos[U];
+    auto fetch = [&](uint32_t t0) {
+        const uint32_t tl = t0 + (lane & 3u) < a.tiles ? t0 + (lane & 3u) : a.tiles - 1;
+        const uint32_t start = h[tl], end = h[a.tiles + tl];
 #pragma unroll
-    for (int j = 0; j < V; j += 16 / (int)sizeof(A)) {
-        u32x4 w;
-        __builtin_memcpy(&w, &x[j], 16);
-        *GLOBAL_PTR(u32x4, p + j * sizeof(A)) = w;
+        for (int u = 0; u < U; u++) {
+            const uint32_t s = __builtin_amdgcn_readlane(start, u);
+            len[u] = t0 + u < to ? __builtin_amdgcn_readlane(end, u) - s : 0;
+            at[u] = (t0 + u) * NBO_SPLIT_TILE + s;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) { // (behind the segment: its first id again, or the last of all)
+            const uint32_t p = at[u] + (lane < len[u] ? lane : 0), q = p < a.n ? p : a.n - 1;
+            key[u] = keys[q] - lo;
+            pos[u] = poss[q];
+        }
+    };
+    auto place = [&](uint32_t r, uint32_t p, uint64_t in) {
+        const uint32_t to_at = place_keys(mine, r, in, a.shift);
+        if (in >> lane & 1) {
+            GLOBAL_PTR(uint32_t, a.keys_out)[to_at] = r + lo;
+            GLOBAL_PTR(uint32_t, a.pos_out)[to_at] = p;
+        }
+    };
+    // what a segment has behind its first 64 (a hot row, padding), again four blocks at a time
+    auto behind = [&](uint32_t first, uint32_t n, auto &&each) {
+        for (uint32_t o = 64; o < n; o += 64 * U) {
+            uint32_t k[U], p[U];
+#pragma unroll
+            for (int j = 0; j < U; j++) {
+                const uint32_t q = first + (o + j * 64 + lane < n ? o + j * 64 + lane : 0);
+                k[j] = keys[q] - lo;
+                p[j] = poss[q];
+            }
+#pragma unroll
+            for (int j = 0; j < U; j++)
+                if (o + j * 64 < n) each(k[j], p[j], __builtin_amdgcn_ballot_w64(o + j * 64 + lane < n));
+        }
+    };
+    if (from < to) fetch(from);
+    __syncthreads();
+    for (uint32_t t0 = from; t0 < to; t0 += U) {
+        if (t0 > from) fetch(t0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (len[u] == 0) continue;
+            count_keys(mine, key[u], __builtin_amdgcn_ballot_w64(lane < len[u]));
+            behind(at[u], len[u], [&](uint32_t r, uint32_t, uint64_t in) { count_keys(mine, r, in); });
+        }
     }
-}
-template <typename A, int V> DEV void load_slot(const char *p, A (&x)[V])
-{
+    starts_of_keys<WAVES>(a, lo, count, range, below, wsum, wbelow);
+    for (uint32_t t0 = from; t0 < to; t0 += U) {
+        if (per > U) fetch(t0);
 #pragma unroll
-    for (int j = 0; j < V; j += 16 / (int)sizeof(A)) {
-        const u32x4 w = *GLOBAL_PTR(const u32x4, p + j * sizeof(A));
-        __builtin_memcpy(&x[j], &w, 16);
+        for (int u = 0; u < U; u++) {
+            if (len[u] == 0) continue;
+            place(key[u], pos[u], __builtin_amdgcn_ballot_w64(lane < len[u]));
+            behind(at[u], len[u], place);
+        }
     }
 }
 
+// After the radix passes: zeros in the rows no id names, four rows to a wave.
 // first place in keys[lo .. hi) whose key is not below `key`
 DEV uint32_t lower_bound(const uint32_t *keys, uint32_t lo, uint32_t hi, uint32_t key)
 {
@@ -511,101 +771,230 @@ DEV uint32_t lower_bound_wave(const uint32_t *keys, uint32_t n, uint32_t key)
     return lo;
 }
 
-// Zeros in the rows from..from + 63 at most whose bit in `named` is not set, by the whole workgroup.
-DEV void clear_rows(const NboEmbedGradArgs &a, uint32_t from, uint32_t count, uint64_t named)
+extern "C" __global__ __launch_bounds__(NBO_OPS_BLOCK) void nbo_order_clear(const NboOrderArgs a)
 {
-    for (uint32_t r = 0; r < count; r++) {
-        if (named >> r & 1) continue;
-        char *p = (char *)a.grad + (uint64_t)(from + r) * a.grad_stride;
-        const u32x4 z = 0;
-        const uint64_t nvec = a.row_bytes / 16;
-        for (uint64_t i = threadIdx.x; i < nvec; i += NBO_OPS_BLOCK) *GLOBAL_PTR(u32x4_e, p + i * 16) = z;
-        // what is left is less than a vector: whole elements, two bytes at a time
-        const uint32_t left = (uint32_t)(a.row_bytes - nvec * 16) / 2;
-        if (threadIdx.x < left) *GLOBAL_PTR(uint16_t, p + nvec * 16 + threadIdx.x * 2) = 0;
-    }
-}
-
-DEV void clear_unnamed(const NboEmbedGradArgs &a, uint32_t wg)
-{
-    __shared__ uint64_t named;
+    enum { ROWS = NBO_CLEAR_ROWS };
     const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t from = (uint64_t)wg * a.zero_rows;
+    const uint64_t from = ((uint64_t)folded_workgroup() * (NBO_OPS_BLOCK / 64) + threadIdx.x / 64) * ROWS;
     if (from >= a.rows) return;
-    const uint32_t count = a.rows - from < a.zero_rows ? (uint32_t)(a.rows - from) : a.zero_rows;
-    if (threadIdx.x < 64) {
-        const uint32_t lo = lower_bound_wave(a.keys, a.n, (uint32_t)from);
-        const uint32_t hi = lower_bound_wave(a.keys, a.n, (uint32_t)from + count);
-        bool here = false;
-        if (lo < hi && lane < count) {
-            const uint32_t at = lower_bound(a.keys, lo, hi, (uint32_t)from + lane);
-            here = at < hi && GLOBAL_PTR(const uint32_t, a.keys)[at] == (uint32_t)from + lane;
-        }
-        const uint64_t m = __builtin_amdgcn_ballot_w64(here);
-        if (lane == 0) named = m;
+    const uint32_t count = a.rows - from < ROWS ? (uint32_t)(a.rows - from) : ROWS;
+    const uint32_t lo = lower_bound_wave(a.keys_in, a.n, (uint32_t)from);
+    const uint32_t hi = lower_bound_wave(a.keys_in, a.n, (uint32_t)from + count);
+    bool here = false;
+    if (lo < hi && lane < count) {
+        const uint32_t at = lower_bound(a.keys_in, lo, hi, (uint32_t)from + lane);
+        here = at < hi && GLOBAL_PTR(const uint32_t, a.keys_in)[at] == (uint32_t)from + lane;
     }
-    __syncthreads();
-    clear_rows(a, (uint32_t)from, count, named);
+    const uint64_t named = __builtin_amdgcn_ballot_w64(here);
+    clear_rows(a.clear, from, count, named);
 }
 
-template <int ED, int EG> DEV void embed_sum_body(const NboEmbedGradArgs &a)
+// ---------------------------------------------------------------------------------
+// The sums.  The order is cut into pieces of a.piece tokens; `lanes` lanes, one unit of the row each,
+// walk a piece and add up the rows of dy.  A row of the table all of whose tokens lie in the piece is
+// finished there; the sums of one that began in an earlier piece or goes on into the next are left in
+// the piece's two slots, for the join.  So a row that half the batch names is added up by many
+// waves, and in the same order of additions on every run.
+template <int EG> DEV char *grad_at(const NboEmbedGradArgs &a, uint32_t key, const Span &s)
 {
-    enum { V = Pair<ED, EG>::V, SD = sizeof(typename El<ED>::Bits), U = 8 };
+    return (char *)a.grad + key * a.grad_stride + (uint64_t)s.c0 * sizeof(typename El<EG>::Bits);
+}
+// A finished sum into its row; `g`, when accumulating, is what was there (asked for ahead of the sum).
+template <int EG, int V> DEV void finish_row(const NboEmbedGradArgs &a, uint32_t key, const Span &s, Unit<EG, V> &g,
+                                             typename El<EG>::A (&x)[V])
+{
     typedef typename El<EG>::A A;
-    const uint32_t wg = folded_workgroup();
-    if (wg >= a.sum_wgs) {
-        if (wg - a.sum_wgs < a.zero_wgs) clear_unnamed(a, wg - a.sum_wgs);
-        return;
-    }
-    const uint32_t wave = wg * (NBO_OPS_BLOCK / 64) + threadIdx.x / 64, lane = threadIdx.x & 63u;
-    uint32_t piece, v;
-    if (a.lanes == 64) {
-        piece = wave / a.slabs;
-        v = (wave - piece * a.slabs) * 64 + lane;
+    const A scale = (A)a.scale;
+    if (a.accumulate) {
+        A y[V];
+        g.unpack(y);
+#pragma unroll
+        for (int j = 0; j < V; j++) x[j] = y[j] + scale * x[j];
     } else {
-        piece = wave * (64 / a.lanes) + lane / a.lanes;
-        v = lane % a.lanes;
+#pragma unroll
+        for (int j = 0; j < V; j++) x[j] = scale * x[j];
     }
+    g.pack(x);
+    g.template store<true>(grad_at<EG>(a, key, s), s.skip, s.n);
+}
+template <int EG, int V, bool TINY> DEV void add_to_grad(const NboEmbedGradArgs &a, uint32_t key, const Span &s,
+                                                         typename El<EG>::A (&x)[V])
+{
+    Unit<EG, V> g;
+    if (a.accumulate) g.template load<TINY, false>(grad_at<EG>(a, key, s), s.n);
+    finish_row<EG, V>(a, key, s, g, x);
+}
+
+enum { SLOT_HEAD = 0, SLOT_TAIL = 1 }; // began in an earlier piece / goes on into the next only
+template <typename A, int V> DEV char *slot_at(const NboEmbedGradArgs &a, uint32_t piece, uint32_t slot, uint32_t v)
+{
+    return (char *)a.partial + (((uint64_t)piece * 2 + slot) * a.units + v) * (V * sizeof(A));
+}
+template <typename A, int V> DEV void store_slot(char *p, const A (&x)[V])
+{
+#pragma unroll
+    for (int j = 0; j < V; j += 16 / (int)sizeof(A)) {
+        u32x4 w;
+        __builtin_memcpy(&w, &x[j], 16);
+        *GLOBAL_PTR(u32x4, p + j * sizeof(A)) = w;
+    }
+}
+template <typename A, int V> DEV void load_slot(const char *p, A (&x)[V])
+{
+#pragma unroll
+    for (int j = 0; j < V; j += 16 / (int)sizeof(A)) {
+        const u32x4 w = *GLOBAL_PTR(const u32x4, p + j * sizeof(A));
+        __builtin_memcpy(&x[j], &w, 16);
+    }
+}
+
+// One piece by `lanes` < 64 lanes, for rows of few units: several pieces to a wave.
+template <int ED, int EG, bool TINY> DEV void sum_narrow(const NboEmbedGradArgs &a, uint32_t wave)
+{
+    enum { V = Pair<ED, EG>::V, SD = sizeof(typename El<ED>::Bits), U = 4 };
+    typedef typename El<EG>::A A;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t piece = wave * (64 / a.lanes) + lane / a.lanes, v = lane % a.lanes;
     if (piece >= a.pieces || v >= a.units) return;
     const Span s = unit_span<V>(v, a.cols);
     const uint32_t from = piece * a.piece, to = a.n - from < a.piece ? a.n : from + a.piece;
     auto *keys = GLOBAL_PTR(const uint32_t, a.keys);
     auto *pos = GLOBAL_PTR(const uint32_t, a.pos);
     uint32_t cur = keys[from];
+    if (cur >= a.rows) return; // nothing but padding
     bool head = from > 0 && keys[from - 1] == cur;
     A acc[V];
 #pragma unroll
     for (int j = 0; j < V; j++) acc[j] = (A)0;
-    for (uint32_t i = from; i < to; i++) {
-        const uint32_t key = keys[i];
-        if (key >= a.rows) break; // padding, to the end
-        if (key != cur) {
-            if (head) store_slot<A, V>(slot_at<A, V>(a, piece, SLOT_HEAD, v), acc);
-            else add_to_grad<EG, V>(a, cur, s, acc);
+    for (uint32_t i = from; i < to; i += U) {
+        uint32_t key[U], row[U];
+        Unit<ED, V> d[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t j = i + u < to ? i + u : to - 1;
+            key[u] = keys[j];
+            row[u] = pos[j];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            d[u].template load<TINY, true>((const char *)a.dy + row[u] * a.dy_stride + (uint64_t)s.c0 * SD, s.n);
+            if (i + u >= to) key[u] = a.rows;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (key[u] >= a.rows) break; // padding, to the end
+            if (key[u] != cur) {
+                if (head) store_slot<A, V>(slot_at<A, V>(a, piece, SLOT_HEAD, v), acc);
+                else add_to_grad<EG, V, TINY>(a, cur, s, acc);
+                head = false;
+                cur = key[u];
+#pragma unroll
+                for (int j = 0; j < V; j++) acc[j] = (A)0;
+            }
+            A x[V];
+            d[u].unpack(x);
+#pragma unroll
+            for (int j = 0; j < V; j++) acc[j] += x[j];
+        }
+    }
+    if (head) store_slot<A, V>(slot_at<A, V>(a, piece, SLOT_HEAD, v), acc);
+    else if (to < a.n && keys[to] == cur) store_slot<A, V>(slot_at<A, V>(a, piece, SLOT_TAIL, v), acc);
+    else add_to_grad<EG, V, TINY>(a, cur, s, acc);
+}
+
+// One piece (of at most 64 tokens) and slab of 64 units by a wave.  Lane i holds token i's key and
+// place, so that which token is the last of its row is one mask, and the rows' addresses are scalars.
+// (Asking for what the finished rows hold together with the tokens' rows, instead of at the row's end, measured
+// slower: 34-36 us against 31.4 for 16384 bf16 rows of 4 KiB into f32.)
+template <int ED, int EG> DEV void sum_wide(const NboEmbedGradArgs &a, uint32_t wave)
+{
+    enum { V = Pair<ED, EG>::V, SD = sizeof(typename El<ED>::Bits), U = 8 };
+    typedef typename El<EG>::A A;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t piece = wave / a.slabs, v = (wave - piece * a.slabs) * 64 + lane;
+    if (piece >= a.pieces) return;
+    const uint32_t from = piece * a.piece, len = a.n - from < a.piece ? a.n - from : a.piece;
+    auto *keys = GLOBAL_PTR(const uint32_t, a.keys);
+    const uint32_t at = from + (lane < len ? lane : len - 1);
+    const uint32_t key = keys[at], pos = GLOBAL_PTR(const uint32_t, a.pos)[at];
+    const uint32_t before = keys[from > 0 ? from - 1 : 0], behind = keys[from + len < a.n ? from + len : a.n - 1];
+    const uint32_t cnt = (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(lane < len && key < a.rows)); // padding sorts last
+    if (cnt == 0) return;
+    const uint32_t next = __shfl_down(key, 1);
+    const uint64_t ends = __builtin_amdgcn_ballot_w64(lane < cnt && (lane == cnt - 1 || key != next));
+    bool head = from > 0 && before == (uint32_t)__builtin_amdgcn_readlane(key, 0);
+    const bool tail = cnt == len && from + len < a.n && behind == (uint32_t)__builtin_amdgcn_readlane(key, len - 1);
+    const bool on = v < a.units;
+    const Span s = unit_span<V>(on ? v : a.units - 1, a.cols);
+    A acc[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) acc[j] = (A)0;
+    for (uint32_t i = 0; i < cnt; i += U) {
+        Unit<ED, V> d[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) { // (behind the last token: that one again)
+            const uint32_t l = i + u < cnt ? i + u : cnt - 1;
+            const char *row = (const char *)a.dy + __builtin_amdgcn_readlane(pos, l) * a.dy_stride;
+            d[u].template load<false, true>(row + (uint64_t)s.c0 * SD, s.n);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (i + u >= cnt) break;
+            A x[V];
+            d[u].unpack(x);
+#pragma unroll
+            for (int j = 0; j < V; j++) acc[j] += x[j];
+            if (!(ends >> (i + u) & 1)) continue;
+            if (on) {
+                if (head) store_slot<A, V>(slot_at<A, V>(a, piece, SLOT_HEAD, v), acc);
+                else if (tail && i + u == cnt - 1) store_slot<A, V>(slot_at<A, V>(a, piece, SLOT_TAIL, v), acc);
+                else add_to_grad<EG, V, false>(a, __builtin_amdgcn_readlane(key, i + u), s, acc);
+            }
             head = false;
-            cur = key;
 #pragma unroll
             for (int j = 0; j < V; j++) acc[j] = (A)0;
         }
-        Unit<ED, V> d;
-        A x[V];
-        d.load((const char *)a.dy + pos[i] * a.dy_stride + (uint64_t)s.c0 * SD, s.n);
-        d.unpack(x);
-#pragma unroll
-        for (int j = 0; j < V; j++) acc[j] += x[j];
     }
-    if (cur >= a.rows) return; // nothing but padding
-    if (head) store_slot<A, V>(slot_at<A, V>(a, piece, SLOT_HEAD, v), acc);
-    else if (to < a.n && keys[to] == cur) store_slot<A, V>(slot_at<A, V>(a, piece, SLOT_TAIL, v), acc);
-    else add_to_grad<EG, V>(a, cur, s, acc);
+}
+
+// Zeros in the rows that no id names: one 16-byte store per thread and its wave is gone, through the
+// matrix from the front -- the shape in which this memory takes a fill fastest (6.6 TB/s over 1 GiB; waves that
+// walk ranges of their own 5.0-5.8).
+DEV void clear_unnamed(const NboEmbedGradArgs &a, uint32_t wg)
+{
+    const uint64_t base = (uint64_t)wg * NBO_OPS_BLOCK;
+    if (base + threadIdx.x >= a.clear_units.total) return;
+    uint64_t row;
+    uint32_t v;
+    unit_at(a.clear_units, unit_base(a.clear_units, base), threadIdx.x, &row, &v);
+    if (GLOBAL_PTR(const uint8_t, a.named)[row]) return;
+    char *p = (char *)a.clear.grad + row * a.clear.grad_stride;
+    if (a.clear.row_bytes >= 16) { // (a row's last 16 bytes end with the row)
+        const uint64_t o = (uint64_t)v * 16 + 16 <= a.clear.row_bytes ? (uint64_t)v * 16 : a.clear.row_bytes - 16;
+        __builtin_nontemporal_store((u32x4_e)0, GLOBAL_PTR(u32x4_e, p + o));
+    } else {
+        for (uint32_t o = 0; o < a.clear.row_bytes; o += 2) *GLOBAL_PTR(uint16_t, p + o) = 0;
+    }
+}
+
+template <int ED, int EG, bool TINY> DEV void embed_sum_body(const NboEmbedGradArgs &a)
+{
+    const uint32_t wg = folded_workgroup();
+    if (wg >= a.sum_wgs) {
+        if (a.clear.grad) clear_unnamed(a, wg - a.sum_wgs);
+        return;
+    }
+    const uint32_t wave = wg * (NBO_OPS_BLOCK / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    if (TINY || a.lanes < 64) sum_narrow<ED, EG, TINY>(a, wave);
+    else sum_wide<ED, EG>(a, wave);
 }
 
 // Rows whose tokens span pieces: the workgroups of boundary k (between pieces k and k + 1), one per slab
 // of the row, finish the row that spans it and begins in piece k.  Its sums are piece k's tail and the
 // heads of the pieces behind, as many as begin with its key; the four waves take a run of them each.
-template <int ED, int EG> DEV void embed_join_body(const NboEmbedGradArgs &a)
+template <int ED, int EG, bool TINY> DEV void embed_join_body(const NboEmbedGradArgs &a)
 {
-    enum { V = Pair<ED, EG>::V, WAVES = NBO_OPS_BLOCK / 64 };
+    enum { V = Pair<ED, EG>::V, WAVES = NBO_OPS_BLOCK / 64, U = 8 };
     typedef typename El<EG>::A A;
     __shared__ A part[WAVES][V][64];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -614,30 +1003,40 @@ template <int ED, int EG> DEV void embed_join_body(const NboEmbedGradArgs &a)
     if (k + 1 >= a.pieces) return;
     auto *keys = GLOBAL_PTR(const uint32_t, a.keys);
     const uint64_t edge = (uint64_t)(k + 1) * a.piece;
-    const uint32_t key = keys[edge];
-    if (key >= a.rows || keys[edge - 1] != key) return; // no row spans this boundary
-    if (k > 0 && keys[edge - a.piece - 1] == key) return; // ... or it began earlier
+    // everything there is to know is asked for at once; lane j: the key that piece k + 2 + j begins with
+    auto first_of = [&](uint64_t p) { return keys[(p < a.pieces ? p : a.pieces - 1) * a.piece]; };
+    const uint32_t key = keys[edge], ahead = keys[edge - 1], earlier = keys[k > 0 ? edge - a.piece - 1 : 0];
+    uint32_t later = first_of((uint64_t)k + 2 + lane);
+    if (key >= a.rows || ahead != key) return; // no row spans this boundary
+    if (k > 0 && earlier == key) return;       // ... or it began earlier
     uint32_t last = k + 1; // the last piece that begins with this row (its boundary is inside the row)
     for (;;) {
-        const uint64_t p = (uint64_t)last + 1 + lane;
-        const bool more = p < a.pieces && keys[p * a.piece] == key;
-        const uint64_t m = ~__builtin_amdgcn_ballot_w64(more);
+        const uint64_t m = ~__builtin_amdgcn_ballot_w64((uint64_t)last + 1 + lane < a.pieces && later == key);
         const uint32_t c = m ? (uint32_t)__builtin_ctzll(m) : 64u;
         last += c;
         if (c < 64) break;
+        later = first_of((uint64_t)last + 1 + lane);
     }
     const uint32_t total = last - k, per = (total + WAVES - 1) / WAVES;
+    const Span s = unit_span<V>(v < a.units ? v : a.units - 1, a.cols);
+    Unit<EG, V> g;
+    if (a.accumulate) g.template load<TINY, false>(grad_at<EG>(a, key, s), s.n);
     A acc[V];
 #pragma unroll
     for (int j = 0; j < V; j++) acc[j] = (A)0;
     if (v < a.units) {
         if (wave == 0) load_slot<A, V>(slot_at<A, V>(a, k, SLOT_TAIL, v), acc);
         const uint32_t lo = wave * per, hi = lo + per < total ? lo + per : total;
-        for (uint32_t i = lo; i < hi; i++) {
-            A x[V];
-            load_slot<A, V>(slot_at<A, V>(a, k + 1 + i, SLOT_HEAD, v), x);
+        for (uint32_t i = lo; i < hi; i += U) {
+            A x[U][V];
 #pragma unroll
-            for (int j = 0; j < V; j++) acc[j] += x[j];
+            for (int u = 0; u < U; u++)
+                if (i + u < hi) load_slot<A, V>(slot_at<A, V>(a, k + 1 + i + u, SLOT_HEAD, v), x[u]);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (i + u < hi)
+#pragma unroll
+                    for (int j = 0; j < V; j++) acc[j] += x[u][j];
         }
     }
 #pragma unroll
@@ -648,16 +1047,15 @@ template <int ED, int EG> DEV void embed_join_body(const NboEmbedGradArgs &a)
         for (int w = 1; w < WAVES; w++)
 #pragma unroll
             for (int j = 0; j < V; j++) acc[j] += part[w][j][lane];
-        const Span s = unit_span<V>(v, a.cols);
-        add_to_grad<EG, V>(a, key, s, acc);
+        finish_row<EG, V>(a, key, s, g, acc);
     }
 }
 
 // A few ids: one wave per token and slab.  It reads all ids; unless an earlier token names the same
-// row it adds up the rows of all tokens that do.  The workgroups behind clear the other rows.
-template <int ED, int EG> DEV void embed_direct_body(const NboEmbedGradArgs &a)
+// row it adds up the rows of all tokens that do.  The waves behind clear the rows no token names.
+template <int ED, int EG, bool TINY> DEV void embed_direct_body(const NboEmbedGradArgs &a)
 {
-    enum { V = Pair<ED, EG>::V, SD = sizeof(typename El<ED>::Bits), BLOCKS = NBO_EMBED_DIRECT_MAX / 64 };
+    enum { V = Pair<ED, EG>::V, SD = sizeof(typename El<ED>::Bits), BLOCKS = NBO_EMBED_DIRECT_MAX / 64, U = 4 };
     typedef typename El<EG>::A A;
     const uint32_t wg = folded_workgroup(), lane = threadIdx.x & 63u;
     uint32_t key[BLOCKS];
@@ -667,21 +1065,18 @@ template <int ED, int EG> DEV void embed_direct_body(const NboEmbedGradArgs &a)
         key[b] = i < a.n ? load_key(a.ids, a.ids64, i, a.rows) : 0xFFFFFFFFu;
     }
     if (wg >= a.sum_wgs) {
-        const uint64_t from = (uint64_t)(wg - a.sum_wgs) * a.zero_rows;
-        if (wg - a.sum_wgs >= a.zero_wgs || from >= a.rows) return;
-        const uint32_t count = a.rows - from < a.zero_rows ? (uint32_t)(a.rows - from) : a.zero_rows;
-        uint32_t lo = 0, hi = 0; // bit r: row from + r is named
+        // four rows to a wave
+        const uint64_t from = ((uint64_t)(wg - a.sum_wgs) * (NBO_OPS_BLOCK / 64) + threadIdx.x / 64) * NBO_CLEAR_ROWS;
+        if (from >= a.rows) return;
+        const uint32_t count = a.rows - from < NBO_CLEAR_ROWS ? (uint32_t)(a.rows - from) : NBO_CLEAR_ROWS;
+        uint64_t named = 0;
+        for (uint32_t r = 0; r < count; r++) {
+            uint64_t here = 0;
 #pragma unroll
-        for (int b = 0; b < BLOCKS; b++) {
-            const uint64_t r = (uint64_t)key[b] - from;
-            if (key[b] >= from && r < count) (r < 32 ? lo : hi) |= 1u << (r & 31);
+            for (int b = 0; b < BLOCKS; b++) here |= __builtin_amdgcn_ballot_w64(key[b] == (uint32_t)from + r);
+            named |= (uint64_t)(here != 0) << r;
         }
-#pragma unroll
-        for (int s = 1; s < 64; s *= 2) {
-            lo |= __shfl_xor(lo, s);
-            hi |= __shfl_xor(hi, s);
-        }
-        clear_rows(a, (uint32_t)from, count, (uint64_t)hi << 32 | lo);
+        clear_rows(a.clear, from, count, named);
         return;
     }
     const uint32_t wave = wg * (NBO_OPS_BLOCK / 64) + threadIdx.x / 64;
@@ -701,35 +1096,52 @@ template <int ED, int EG> DEV void embed_direct_body(const NboEmbedGradArgs &a)
     }
     if (!first || v >= a.units) return;
     const Span s = unit_span<V>(v, a.cols);
+    Unit<EG, V> g;
+    if (a.accumulate) g.template load<TINY, false>(grad_at<EG>(a, own, s), s.n);
     A acc[V];
 #pragma unroll
     for (int j = 0; j < V; j++) acc[j] = (A)0;
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++)
-        for (uint64_t m = same[b]; m; m &= m - 1) {
-            const uint64_t i = b * 64 + __builtin_ctzll(m);
-            Unit<ED, V> d;
-            A x[V];
-            d.load((const char *)a.dy + i * a.dy_stride + (uint64_t)s.c0 * SD, s.n);
-            d.unpack(x);
+        for (uint64_t m = same[b]; m;) {
+            Unit<ED, V> d[U];
+            uint32_t got = 0, i = 0;
 #pragma unroll
-            for (int j = 0; j < V; j++) acc[j] += x[j];
+            for (int u = 0; u < U; u++) { // (behind the last token: that one again)
+                if (m) {
+                    i = b * 64 + __builtin_ctzll(m);
+                    m &= m - 1;
+                    got++;
+                }
+                d[u].template load<TINY, true>((const char *)a.dy + i * a.dy_stride + (uint64_t)s.c0 * SD, s.n);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if ((uint32_t)u >= got) break;
+                A x[V];
+                d[u].unpack(x);
+#pragma unroll
+                for (int j = 0; j < V; j++) acc[j] += x[j];
+            }
         }
-    add_to_grad<EG, V>(a, own, s, acc);
+    finish_row<EG, V>(a, own, s, g, acc);
 }
 
 #define NBO_EMBED_GRAD_KERNELS(suffix, ED, EG)                                                                   \
     extern "C" __global__ __launch_bounds__(NBO_OPS_BLOCK) void nbo_embed_sum_##suffix(const NboEmbedGradArgs a) \
     {                                                                                                            \
-        embed_sum_body<ED, EG>(a);                                                                               \
+        if (a.cols >= (uint32_t)Pair<ED, EG>::V) embed_sum_body<ED, EG, false>(a);                               \
+        else embed_sum_body<ED, EG, true>(a);                                                                     \
     }                                                                                                            \
     extern "C" __global__ __launch_bounds__(NBO_OPS_BLOCK) void nbo_embed_join_##suffix(const NboEmbedGradArgs a)\
     {                                                                                                            \
-        embed_join_body<ED, EG>(a);                                                                              \
+        if (a.cols >= (uint32_t)Pair<ED, EG>::V) embed_join_body<ED, EG, false>(a);                               \
+        else embed_join_body<ED, EG, true>(a);                                                                     \
     }                                                                                                            \
     extern "C" __global__ __launch_bounds__(NBO_OPS_BLOCK) void nbo_embed_direct_##suffix(const NboEmbedGradArgs a) \
     {                                                                                                            \
-        embed_direct_body<ED, EG>(a);                                                                            \
+        if (a.cols >= (uint32_t)Pair<ED, EG>::V) embed_direct_body<ED, EG, false>(a);                               \
+        else embed_direct_body<ED, EG, true>(a);                                                                     \
     }
 NBO_EMBED_GRAD_KERNELS(f32, NBO_F32, NBO_F32)
 NBO_EMBED_GRAD_KERNELS(bf16, NBO_BF16, NBO_BF16)
@@ -761,27 +1173,14 @@ DEV void philox(uint32_t block, uint32_t site, const NboRngDev &r, uint32_t (&w)
     w[3] = c3;
 }
 
-template <int E> DEV void dropout_body(const NboDropoutArgs &a)
+// One unit of V elements per thread.  PART: the last one of a row or the matrix, which has fewer.
+template <int E, bool PART, bool ONCE> DEV void dropout_unit(const NboDropoutArgs &a, uint64_t row, uint64_t c, uint64_t e, uint32_t n)
 {
     enum { V = Pair<E, E>::V, SZ = sizeof(typename El<E>::Bits) };
     typedef typename El<E>::A A;
-    const uint64_t base = (uint64_t)folded_workgroup() * NBO_OPS_BLOCK;
-    const uint64_t unit = base + threadIdx.x;
-    if (unit >= a.u.total) return;
-    uint64_t row = 0, c = unit * V, e = c; // element `e` of the matrix, at column c of `row`
-    Span s = {0, 0, V};
-    if (a.flat) {
-        s.n = a.n - e < V ? (uint32_t)(a.n - e) : V;
-    } else {
-        uint32_t v;
-        unit_at(a.u, unit_base(a.u, base), threadIdx.x, &row, &v);
-        c = (uint64_t)v * V;
-        e = row * a.cols + c;
-        s.n = a.cols - c < V ? (uint32_t)(a.cols - c) : V;
-    }
     Unit<E, V> x, y;
-    x.load((const char *)a.x + row * a.x_stride + c * SZ, s.n);
-    if (a.residual) y.load((const char *)a.residual + row * a.residual_stride + c * SZ, s.n);
+    x.template load<PART, ONCE>((const char *)a.x + row * a.x_stride + c * SZ, n);
+    if (a.residual) y.template load<PART, ONCE>((const char *)a.residual + row * a.residual_stride + c * SZ, n);
     const NboRngDev rng = *a.rng;
     uint32_t bits[V]; // each element's sixteen
     uint32_t w[4];
@@ -828,7 +1227,29 @@ template <int E> DEV void dropout_body(const NboDropoutArgs &a)
         for (int j = 0; j < V; j++) f[j] = g[j] + f[j];
     }
     x.pack(f);
-    x.store((char *)a.out + row * a.out_stride + c * SZ, 0, s.n);
+    x.template store<ONCE>((char *)a.out + row * a.out_stride + c * SZ, 0, n);
+}
+
+template <int E> DEV void dropout_body(const NboDropoutArgs &a)
+{
+    enum { V = Pair<E, E>::V };
+    const uint64_t base = (uint64_t)folded_workgroup() * NBO_OPS_BLOCK;
+    const uint64_t unit = base + threadIdx.x;
+    if (unit >= a.u.total) return;
+    uint64_t row = 0, c = unit * V, e = c; // element `e` of the matrix, at column c of `row`
+    uint32_t n;
+    if (a.flat) {
+        n = a.n - e < V ? (uint32_t)(a.n - e) : V;
+    } else {
+        uint32_t v;
+        unit_at(a.u, unit_base(a.u, base), threadIdx.x, &row, &v);
+        c = (uint64_t)v * V;
+        e = row * a.cols + c;
+        n = a.cols - c < V ? (uint32_t)(a.cols - c) : V;
+    }
+    if (n != V) dropout_unit<E, true, false>(a, row, c, e, n);
+    else if (a.once) dropout_unit<E, false, true>(a, row, c, e, V);
+    else dropout_unit<E, false, false>(a, row, c, e, V);
 }
 
 #define NBO_DROPOUT_KERNEL(name, E)                                                           \

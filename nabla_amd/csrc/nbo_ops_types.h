@@ -5,6 +5,8 @@
 
 #include <stdint.h>
 
+// Units per thread of the lookup (65536 rows of 8 KiB: one 181 us, two 149, four 138, eight 154).
+#define NBO_EMBED_UNITS 4
 #define NBO_OPS_BLOCK 256u // threads of every operator kernel but the ordering ones
 
 // The generator's state in device memory.
@@ -48,6 +50,8 @@ struct NboDropoutArgs {
     uint32_t site;
     uint32_t thr; // 0 .. 65536
     uint32_t flat; // rows are adjacent: units run through the matrix
+    uint32_t once; // more than the last level of cache holds: stream past it
+    uint32_t pad;
 };
 
 struct NboRngAdvanceArgs {
@@ -58,27 +62,48 @@ struct NboRngAdvanceArgs {
 // ---- the gradient of the embedding ------------------------------------------------------
 // Keys: the ids, with every id outside the table replaced by `rows`, so that padding sorts last.
 
-// All-pairs ranking: one launch orders up to NBO_RANK_MAX ids.
-#define NBO_RANK_MAX 16384u
-#define NBO_RANK_BLOCK 1024u
+// Order by ranges: one launch, every workgroup reads all ids; threads, and the most ids (they stay in
+// registers) and keys per workgroup (LDS: 4 bytes for each wave and key).
+#define NBO_RANGE_BLOCK 1024u
+#define NBO_RANGE_IDS 8192u
+#define NBO_RANGE_KEYS 960u
 // Radix passes: ids per workgroup and the widest digit.
 #define NBO_RADIX_TILE 4096u
 #define NBO_RADIX_BLOCK 512u
 #define NBO_RADIX_BITS 10u
+// Split and merge: ids per tile, and the widest range of keys, as a power of two (LDS of the merge: 4 bytes
+// for each wave and key).
+#define NBO_SPLIT_TILE 1024u
+#define NBO_SPLIT_SHIFT 9u
 // Up to this many ids the gradient is one launch that needs no order.
 #define NBO_EMBED_DIRECT_MAX 256u
 
+// Rows to clear: those of grad that no id names (grad null: none).
+#define NBO_CLEAR_ROWS 4u // per wave, where it has to find out which
+struct NboClearArgs {
+    void *grad;
+    uint64_t grad_stride, row_bytes;
+};
+
+// Largest table for which the ordering launches note the rows that have ids (one byte each); the radix passes
+// do not, and a launch of its own looks the rows up.
+#define NBO_NAMED_ROWS (1u << 21)
+
 struct NboOrderArgs {
+    NboClearArgs clear;    // nbo_order_clear
+    uint8_t *named;        // [rows] or null: whether a row has ids
     const void *ids;       // the caller's (first pass), or null: keys_in / pos_in
     const uint32_t *keys_in, *pos_in;
     uint32_t *keys_out, *pos_out;
-    uint32_t *hist;        // [digits][tiles]
+    uint32_t *hist;        // [digits][tiles]; of the split: [digits + 1][tiles]
     uint32_t *totals;      // [digits]
     uint32_t n;
     uint32_t rows;
     uint32_t ids64;
     uint32_t tiles;
-    uint32_t shift, digits; // this pass's digit: (key >> shift) & (digits - 1)
+    uint32_t shift, digits; // this pass's digit: (key >> shift) & (digits - 1); of the split: key >> shift
+    uint32_t range;         // keys per workgroup (order by ranges)
+    uint32_t pad;
 };
 
 struct NboEmbedGradArgs {
@@ -88,18 +113,18 @@ struct NboEmbedGradArgs {
     const uint32_t *keys, *pos;   // in table order
     void *partial;                // [pieces][2][units * VEC] sums of rows that span pieces
     uint64_t dy_stride, grad_stride; // bytes
-    uint64_t row_bytes;           // of a row of grad
+    NboClearArgs clear;
+    NboUnits clear_units;         // 16 bytes each
+    const uint8_t *named;
     double scale;
     uint32_t n, rows, cols;
     uint32_t units;               // per row
     uint32_t lanes;               // lanes that work on one piece: 64, or a power of two that holds `units`
     uint32_t slabs;               // waves per piece (lanes == 64)
     uint32_t piece, pieces;       // ids per piece, pieces
-    uint32_t sum_wgs, zero_wgs;   // workgroups that add, workgroups that clear rows no id names
-    uint32_t zero_rows;           // rows per clearing workgroup, at most 64
+    uint32_t sum_wgs;             // workgroups that add; those behind them clear
     uint32_t accumulate;
     uint32_t ids64;
-    uint32_t pad;
 };
 
 #endif

@@ -32,39 +32,40 @@ from . import _lib
 from .optim import _call, _dtype_code, _shape2
 
 
+_dtype_codes = {}  # by dtype object: spares the smallest calls the name's parsing
+
+
 def _matrix(t) -> _lib.Matrix:
-    shape = t.shape
-    strides = t.stride() if hasattr(t, "stride") else None
-    if len(shape) == 2:
-        rows, cols = shape
-        if strides is None:
-            stride = cols
-        else:
-            stride, unit = strides
-            if unit != 1 and cols > 1:
-                raise ValueError("the elements of a row must be adjacent")
-    else:
+    try:
+        rows, cols = t.shape
+        stride, unit = t.stride()
+    except (AttributeError, ValueError):  # no strides, or not two dimensions
+        if hasattr(t, "is_contiguous") and not t.is_contiguous():
+            raise ValueError("a strided tensor must have two dimensions") from None
         rows, cols = _shape2(t)
-        if strides is not None and not t.is_contiguous():
-            raise ValueError("a strided tensor must have two dimensions")
-        stride = cols
-    return _lib.Matrix(t.data_ptr(), rows, cols, stride, _dtype_code(t), 0)
+        stride, unit = cols, 1
+    if unit != 1 and cols > 1:
+        raise ValueError("the elements of a row must be adjacent")
+    code = _dtype_codes.get(t.dtype)
+    if code is None:
+        code = _dtype_codes[t.dtype] = _dtype_code(t)
+    return _lib.Matrix(t.data_ptr(), rows, cols, stride, code, 0)
+
+
+_id_codes = {}
 
 
 def _ids(t) -> _lib.Ids:
-    name = str(t.dtype)
-    if name.endswith("int64") and not name.endswith("uint64"):
-        kind = _lib.ID_I64
-    elif name.endswith("int32") and not name.endswith("uint32"):
-        kind = _lib.ID_I32
-    else:
-        raise TypeError(f"ids are int32 or int64, not {name}")
+    code = _id_codes.get(t.dtype)
+    if code is None:
+        name = str(t.dtype).rsplit(".", 1)[-1]
+        if name not in ("int32", "int64"):
+            raise TypeError(f"ids are int32 or int64, not {name}")
+        code = _id_codes[t.dtype] = _lib.ID_I64 if name == "int64" else _lib.ID_I32
     if hasattr(t, "is_contiguous") and not t.is_contiguous():
         raise ValueError("ids must be contiguous")
-    n = 1
-    for x in t.shape:
-        n *= int(x)
-    return _lib.Ids(t.data_ptr(), n, kind, 0)
+    rows, cols = _shape2(t)
+    return _lib.Ids(t.data_ptr(), rows * cols, code, 0)
 
 
 def embedding(table, ids, out, scale: float = 1.0, add=None) -> None:

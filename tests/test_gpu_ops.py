@@ -195,9 +195,12 @@ def test_embedding_grad_of_one_row_and_of_padding_alone(gpu, n):
 
 
 @pytest.mark.parametrize("rows,n", [(1, 300), (2, 20000), (255, 20000), (256, 20000), (1023, 20000), (1024, 20000),
-                                    ((1 << 20) - 1, 20000), (1 << 20, 20000), ((1 << 21) + 5, 30000), (3_000_017, 5000)])
+                                    ((1 << 20) - 1, 20000), (1 << 20, 20000), ((1 << 21) + 5, 30000), (3_000_017, 5000),
+                                    (1, 140000), (2, 140000), (255, 140001), (256, 140000), (1023, 139999),
+                                    (1024, 140000), (50257, 300000)])
 def test_embedding_grad_table_sizes(gpu, rows, n):
-    """Around the digit widths of the radix passes; the last rows of the table among the ids."""
+    """Around the ways to order the ids (key ranges; radix passes for many ids or rows) and the digit widths
+    of the passes; the last rows of the table among the ids."""
     ws = ops.EmbeddingWorkspace(n, 4)
     ids = rand_ids(n, rows, 3, 0.05)
     ids[::7] = rows - 1
