@@ -62,7 +62,7 @@ int nbo_embedding_ws_destroy(nbo_embedding_ws *ws);
 /* The gradient of nbo_embedding with respect to the table:
  *   grad[v] = (accumulate ? grad[v] : 0) + scale * sum of grad_out[t] over the t with ids[t] == v
  * With accumulate == 0 every row is written, zeros where no id names it; otherwise the rows no id
- * names are not touched.  Rows of grad_out whose id is outside the table are not read.  Sums are
+ * names are not touched.  What rows of grad_out hold whose id is outside the table does not matter.  Sums are
  * f32 (f64 lists: f64), over the tokens in a fixed order -- the same bits on every run -- and
  * rounded once, to grad's type: grad_out's, or f32 over bf16 / f16.  (With respect to `add` the
  * gradient is grad_out itself.)  grad may not overlap grad_out or the ids.  Asynchronous. */

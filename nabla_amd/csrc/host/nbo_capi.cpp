@@ -34,7 +34,7 @@ bool pointer_checks_enabled()
     return on;
 }
 
-void check_device_address(const void *ptr, uint64_t bytes, const char *what)
+void check_device_address(const void *ptr, uint64_t bytes, const char *what, int device)
 {
     char where[96];
     std::snprintf(where, sizeof(where), "%s at %p", what, ptr);
@@ -43,6 +43,9 @@ void check_device_address(const void *ptr, uint64_t bytes, const char *what)
     if (e != hipSuccess) (void)hipGetLastError();
     if (e != hipSuccess || attr.type == hipMemoryTypeUnregistered)
         fail(NBO_ERR_ARG, std::string(where) + ": not memory the HIP runtime knows (a host pointer?)");
+    if (device >= 0 && attr.type == hipMemoryTypeDevice && attr.device != device)
+        fail(NBO_ERR_ARG, std::string(where) + ": memory of device " + std::to_string(attr.device) +
+                              ", the library works on device " + std::to_string(device));
     hipDeviceptr_t base = nullptr;
     size_t size = 0;
     if (hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)ptr) != hipSuccess) {

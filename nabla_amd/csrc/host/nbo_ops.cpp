@@ -113,12 +113,12 @@ bool same(const nbo_matrix &a, const nbo_matrix &b)
 void check_address(const nbo_matrix &m, const char *what)
 {
     const uint64_t bytes = extent(m);
-    if (bytes && pointer_checks_enabled()) check_device_address(m.data, bytes, what);
+    if (bytes && pointer_checks_enabled()) check_device_address(m.data, bytes, what, Runtime::get().device());
 }
 
 void check_address(const nbo_ids &ids)
 {
-    if (ids.n && pointer_checks_enabled()) check_device_address(ids.data, id_bytes(ids), "ids");
+    if (ids.n && pointer_checks_enabled()) check_device_address(ids.data, id_bytes(ids), "ids", Runtime::get().device());
 }
 
 NboUnits units_of(uint64_t rows, uint64_t per_row)

@@ -2,8 +2,9 @@
 // and dropout from a counter-based generator.  A code object of its own beside the optimizer's.
 //
 //   nbo_embed_*        out[t] = add[t] + scale * table[ids[t]]
-//   nbo_order_range    the ids in table order, in one launch (up to some 10^5 ids)
-//   nbo_order_split / _merge   ... in two (more ids), nbo_order_hist / _scan / _scatter   ... by radix passes (more rows)
+//   nbo_order_range    the ids in table order, in one launch (up to 8192 ids)
+//   nbo_order_split / _merge             ... in two (more ids)
+//   nbo_order_hist / _scan / _scatter    ... by radix passes (tables of more than half a million rows)
 //   nbo_order_clear    zeros in the rows no id names, behind the radix passes
 //   nbo_embed_sum_*    grad[v] (+)= scale * sum of the rows of dy that name v, in pieces of the order; zeros in the
 //                      rows no id names
@@ -195,13 +196,8 @@ DEV void unit_at(const NboUnits &u, const UnitBase &b, uint32_t x, uint64_t *row
     *v = y - q * u.per_row;
 }
 
-// the id of token t as a row of the table, or `rows` for an id outside it
-DEV uint32_t load_key(const void *ids, uint32_t ids64, uint64_t t, uint32_t rows)
-{
-    const uint64_t id = ids64 ? GLOBAL_PTR(const uint64_t, ids)[t] : (uint64_t)GLOBAL_PTR(const uint32_t, ids)[t];
-    return id < rows ? (uint32_t)id : rows;
-}
-// ... of U tokens at once: a branch that used what it loads would wait for it, so the keys come after all loads
+// The ids of U tokens as rows of the table, `rows` for one outside it.  (All loads first, then the keys: a
+// branch that used what it loads would wait for it.)
 template <int U> DEV void load_keys(const void *ids, uint32_t ids64, const uint64_t (&t)[U], uint32_t rows, uint32_t (&key)[U])
 {
     uint64_t id[U];
@@ -394,17 +390,6 @@ template <int WAVES> DEV void starts_of_keys(const NboOrderArgs &a, uint32_t lo,
     __syncthreads();
 }
 
-template <int U> DEV void range_keys(const NboOrderArgs &a, uint32_t blk, uint32_t (&key)[U])
-{
-    uint64_t t[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) { // (behind the last id: that one again)
-        const uint64_t i = (uint64_t)(blk + u) * 64 + (threadIdx.x & 63u);
-        t[u] = i < a.n ? i : a.n - 1;
-    }
-    load_keys<U>(a.ids, a.ids64, t, a.rows, key);
-}
-
 // Zeros in `bytes` bytes (an even number) at an even address, by a whole wave: two bytes at a time up to
 // the first 16-byte boundary and behind the last.
 DEV void clear_bytes(char *p, uint64_t bytes)
@@ -479,22 +464,32 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_range(co
 // ---------------------------------------------------------------------------------
 // Table order by stable radix passes of up to ten bits, least significant first.  Per pass: how often
 // each digit occurs in each tile; the running sums over the tiles, per digit; every id to its place.
-DEV uint32_t order_key(const NboOrderArgs &a, uint32_t i)
+template <int N> DEV void order_keys(const NboOrderArgs &a, const uint64_t (&t)[N], uint32_t (&key)[N])
 {
-    return a.keys_in ? GLOBAL_PTR(const uint32_t, a.keys_in)[i] : load_key(a.ids, a.ids64, i, a.rows);
+    if (!a.keys_in) {
+        load_keys<N>(a.ids, a.ids64, t, a.rows, key);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++) key[k] = GLOBAL_PTR(const uint32_t, a.keys_in)[t[k]];
+    }
 }
 
 extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_hist(const NboOrderArgs a)
 {
+    enum { ROWS = NBO_RADIX_TILE / NBO_RADIX_BLOCK };
     __shared__ uint32_t count[1u << NBO_RADIX_BITS];
     for (uint32_t d = threadIdx.x; d < a.digits; d += NBO_RADIX_BLOCK) count[d] = 0;
-    __syncthreads();
-    const uint32_t first = blockIdx.x * NBO_RADIX_TILE;
+    const uint32_t first = blockIdx.x * NBO_RADIX_TILE + threadIdx.x;
+    uint64_t t[ROWS];
+    uint32_t key[ROWS];
 #pragma unroll
-    for (uint32_t k = 0; k < NBO_RADIX_TILE / NBO_RADIX_BLOCK; k++) {
-        const uint32_t i = first + k * NBO_RADIX_BLOCK + threadIdx.x;
-        // (counts: the order of these additions changes nothing)
-        if (i < a.n) atomicAdd(&count[(order_key(a, i) >> a.shift) & (a.digits - 1)], 1u);
+    for (int r = 0; r < ROWS; r++) t[r] = first + r * NBO_RADIX_BLOCK < a.n ? first + r * NBO_RADIX_BLOCK : a.n - 1;
+    order_keys<ROWS>(a, t, key);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+        const uint64_t on = __builtin_amdgcn_ballot_w64(first + r * NBO_RADIX_BLOCK < a.n);
+        if (on) count_keys(count, (key[r] >> a.shift) & (a.digits - 1), on);
     }
     __syncthreads();
     for (uint32_t d = threadIdx.x; d < a.digits; d += NBO_RADIX_BLOCK)
@@ -557,15 +552,21 @@ extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_scatter(
         for (int w = 0; w < WAVES; w++) count[w][d] = 0;
     const uint32_t first = blockIdx.x * NBO_RADIX_TILE + wave * (ROWS * 64) + lane;
     uint32_t key[ROWS], pos[ROWS], rank[ROWS], digit[ROWS];
+    uint64_t t[ROWS];
     bool on[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; r++) {
-        const uint32_t i = first + r * 64;
-        on[r] = i < a.n;
-        key[r] = on[r] ? order_key(a, i) : 0;
-        pos[r] = on[r] ? (a.pos_in ? GLOBAL_PTR(const uint32_t, a.pos_in)[i] : i) : 0;
-        digit[r] = (key[r] >> a.shift) & (a.digits - 1);
+        on[r] = first + r * 64 < a.n;
+        t[r] = on[r] ? first + r * 64 : a.n - 1;
+        pos[r] = first + r * 64;
     }
+    order_keys<ROWS>(a, t, key);
+    if (a.pos_in) {
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) pos[r] = GLOBAL_PTR(const uint32_t, a.pos_in)[t[r]];
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) digit[r] = (key[r] >> a.shift) & (a.digits - 1);
     __syncthreads();
     rank_digits<ROWS>(count[wave], digit, on, a.digits, rank);
     __syncthreads();
@@ -741,8 +742,7 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
     }
 }
 
-// After the radix passes: zeros in the rows no id names, four rows to a wave.
-// first place in keys[lo .. hi) whose key is not below `key`
+// First place in keys[lo .. hi) whose key is not below `key`
 DEV uint32_t lower_bound(const uint32_t *keys, uint32_t lo, uint32_t hi, uint32_t key)
 {
     while (lo < hi) {
@@ -771,6 +771,7 @@ DEV uint32_t lower_bound_wave(const uint32_t *keys, uint32_t n, uint32_t key)
     return lo;
 }
 
+// After the radix passes: zeros in the rows no id names, a few rows to a wave.
 extern "C" __global__ __launch_bounds__(NBO_OPS_BLOCK) void nbo_order_clear(const NboOrderArgs a)
 {
     enum { ROWS = NBO_CLEAR_ROWS };
@@ -1058,14 +1059,19 @@ template <int ED, int EG, bool TINY> DEV void embed_direct_body(const NboEmbedGr
     enum { V = Pair<ED, EG>::V, SD = sizeof(typename El<ED>::Bits), BLOCKS = NBO_EMBED_DIRECT_MAX / 64, U = 4 };
     typedef typename El<EG>::A A;
     const uint32_t wg = folded_workgroup(), lane = threadIdx.x & 63u;
-    uint32_t key[BLOCKS];
+    uint32_t key[BLOCKS] = {};
+    if (a.n > 0) {
+        uint64_t t[BLOCKS];
 #pragma unroll
-    for (int b = 0; b < BLOCKS; b++) {
-        const uint32_t i = b * 64 + lane;
-        key[b] = i < a.n ? load_key(a.ids, a.ids64, i, a.rows) : 0xFFFFFFFFu;
+        for (int b = 0; b < BLOCKS; b++) t[b] = b * 64 + lane < a.n ? b * 64 + lane : a.n - 1;
+        load_keys<BLOCKS>(a.ids, a.ids64, t, a.rows, key);
     }
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++)
+        if (b * 64 + lane >= a.n) key[b] = 0xFFFFFFFFu;
     if (wg >= a.sum_wgs) {
-        // four rows to a wave
+        if (!a.clear.grad) return; // the unused end of a folded grid
+        // a few rows to a wave
         const uint64_t from = ((uint64_t)(wg - a.sum_wgs) * (NBO_OPS_BLOCK / 64) + threadIdx.x / 64) * NBO_CLEAR_ROWS;
         if (from >= a.rows) return;
         const uint32_t count = a.rows - from < NBO_CLEAR_ROWS ? (uint32_t)(a.rows - from) : NBO_CLEAR_ROWS;

@@ -104,8 +104,8 @@ def embedding_grad(grad_out, ids, grad, workspace: EmbeddingWorkspace, scale: fl
     grad[v] = (grad[v] if accumulate else 0) + scale * sum of grad_out[t] over ids[t] == v.
 
     Without `accumulate` every row of `grad` is written, zeros where no id names it; with it the
-    rows no id names are not touched.  Rows of `grad_out` whose id is outside the table are not
-    read.  `grad` has grad_out's type, or f32 under bf16 / f16.  Sums are f32 (f64: f64) in a fixed
+    rows no id names are not touched.  What rows of `grad_out` hold whose id is outside the table does
+    not matter.  `grad` has grad_out's type, or f32 under bf16 / f16.  Sums are f32 (f64: f64) in a fixed
     order, the same bits on every run, rounded once."""
     _call(_lib.load().nbo_embedding_grad(_matrix(grad_out), _ids(ids), scale, 1 if accumulate else 0, _matrix(grad),
                                          workspace._h))

@@ -19,6 +19,10 @@ advance on a skipped step.  With accumulation, steps 1-3 are one pass over the g
 squares for the clip) with the reference's synchronous decision after it, and step 4 is
 clip + update + zeroing in one kernel (`fused_step_norm`); with a scaler *and* a nan policy
 the two decisions stay separate entry points in the reference's order.
+
+A generator given with `with_rng` (nabla_amd.ops.DropoutRng) is advanced once per micro-batch,
+whatever became of it, so that the dropouts of the next one draw other masks; its step is
+`state.rng_state`, which checkpoints carry (checkpoint.rs:107-150, `rng.state`).
 """
 from __future__ import annotations
 
@@ -49,6 +53,7 @@ class TrainerTail:
         self.scaler: Optional[nb.GradScaler] = None
         self.grad_clip: Optional[float] = None
         self.nan_policy: Optional[GradNanPolicy] = None
+        self.rng = None
         self.state = TrainState(epoch=0, step=0, grad_accum=1, rng_state=None)
         self._accum = None
         self._accum_count = 0
@@ -74,8 +79,26 @@ class TrainerTail:
         self.grad_clip = float(max_norm) if max_norm > 0.0 else None
         return self
 
+    def with_rng(self, rng) -> "TrainerTail":
+        """`rng`: the ops.DropoutRng whose step one micro-batch's forward and backward pass share.
+        Where a checkpoint has left a step in `state`, the generator goes on from there."""
+        self.rng = rng
+        self._load_rng()
+        return self
+
+    def _load_rng(self) -> None:
+        if self.rng is None:
+            return
+        at = self.rng.state()
+        if self.state.rng_state is None:
+            self.state.rng_state = at.step
+        elif at.step != self.state.rng_state:
+            at.step = self.state.rng_state
+            self.rng.load_state(at)
+
     def set_state(self, state: TrainState) -> None:
         self.state = state
+        self._load_rng()
 
     def schedule_state(self) -> Optional[ScheduleState]:
         return self.schedule
@@ -89,6 +112,15 @@ class TrainerTail:
         """Consume one micro-batch's gradients; returns True if the optimizer stepped.  The
         reference unscales the gradients in place on the way; here they are only read (nothing
         uses them afterwards), except on the path with both a scaler and a nan policy."""
+        if self.rng is None:
+            return self._consume(grads)
+        try:
+            return self._consume(grads)
+        finally:  # the micro-batch is over, stepped, skipped or in error
+            self.rng.advance()
+            self.state.rng_state = (self.state.rng_state + 1) % (1 << 64)
+
+    def _consume(self, grads) -> bool:
         grads = grads if isinstance(grads, nb.TensorList) else list(grads)
         fusable = self.state.grad_accum == 1 and not (self.scaler and self.nan_policy)
         if fusable:

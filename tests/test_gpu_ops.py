@@ -195,7 +195,8 @@ def test_embedding_grad_of_one_row_and_of_padding_alone(gpu, n):
 
 
 @pytest.mark.parametrize("rows,n", [(1, 300), (2, 20000), (255, 20000), (256, 20000), (1023, 20000), (1024, 20000),
-                                    ((1 << 20) - 1, 20000), (1 << 20, 20000), ((1 << 21) + 5, 30000), (3_000_017, 5000),
+                                    ((1 << 20) - 1, 20000), (1 << 20, 20000), ((1 << 21) + 5, 30000), (3_000_017, 5000), (1 << 21, 8192),
+                                    ((1 << 21) + 1, 8192), ((1 << 19) - 1, 8193), (1 << 19, 8193),
                                     (1, 140000), (2, 140000), (255, 140001), (256, 140000), (1023, 139999),
                                     (1024, 140000), (50257, 300000)])
 def test_embedding_grad_table_sizes(gpu, rows, n):
@@ -585,3 +586,75 @@ def test_inputs_on_another_stream(gpu):
             assert torch.equal(out, want)
     finally:
         _lib.check(lib.nbo_set_stream(None))
+
+
+def test_training_goes_on_from_a_checkpoint_with_the_same_masks(gpu, tmp_path):
+    """Three micro-batches through TrainerTail, saved after the first and resumed with fresh objects: the
+    masks, gradients and parameters of the others are the same bits."""
+    from nabla_amd import checkpoint as ck
+    from nabla_amd.trainer import TrainerTail
+
+    def micro_batch(b, tail):
+        ops.embedding(b.params[0], b.tokens, b.x)
+        ops.dropout(b.x, 0.3, b.rng, 2, b.x)
+        torch.sub(b.x, b.target, out=b.dx)
+        ops.dropout_grad(b.dx, 0.3, b.rng, 2, b.dx)
+        ops.embedding_grad(b.dx, b.tokens, b.grads[0], b.ws)
+        tail.after_backward(b.grads)
+
+    a = _InputBlock(5)
+    ta = TrainerTail(a.opt, a.params).with_rng(a.rng).with_grad_clip(1.0)
+    micro_batch(a, ta)
+    assert a.rng.state().step == 18 == ta.state.rng_state
+    names = ["wte", "wpe"]
+    ck.save_checkpoint(str(tmp_path), list(zip(names, a.params)), a.opt, None, None, ta.state)
+    b = _InputBlock(5)  # another process: initial values again
+    params, state, _ = ck.load_checkpoint(str(tmp_path), b.opt)
+    for (name, value), p in zip(params, b.params):
+        p.copy_(torch.as_tensor(value).to(p))
+    b.rng.load_state(ops.DropoutRngState(5, 0))
+    tb = TrainerTail(b.opt, b.params).with_rng(b.rng).with_grad_clip(1.0)
+    tb.set_state(state)
+    for _ in range(2):
+        micro_batch(a, ta)
+        micro_batch(b, tb)
+        assert torch.equal(a.x, b.x) and a.rng.state() == b.rng.state()
+        assert torch.equal(a.params[0], b.params[0]) and torch.equal(a.grads[0], b.grads[0])
+
+
+def test_cpp_program(gpu):
+    import os
+    import subprocess
+
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "test_ops.bin")
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "0 failure(s)" in r.stdout, r.stdout + r.stderr
+
+
+def test_grids_folded_into_two_dimensions(gpu):
+    """Launches of more than 2^24 - 1 workgroups are folded; NBO_GRID_X_MAX=7 in the environment (a test
+    hook of the runtime) folds every one here, the last grid row partly unused."""
+    import os
+    import subprocess
+    import sys
+
+    code = r"""
+import torch
+from nabla_amd import ops
+from tests import test_gpu_ops as t
+for pair, rows, cols, n in (("bf16", 3000, 513, 100), ("f32", 3000, 77, 2000), ("f16", 2000, 24, 9000),
+                            ("f32", (1 << 21) + 9, 3, 700)):
+    table, add = t.randn(rows, cols, pair, 1), t.randn(n, cols, pair, 2)
+    ids = t.rand_ids(n, rows, 3, 0.1, True)
+    t.check_embedding(table, ids, torch.empty_like(add), 1.5, add)
+    ws = ops.EmbeddingWorkspace(n, cols)
+    for accumulate in (False, True):
+        t.check_grad(add, ids, table, ws, 1.0, accumulate, pair)
+    t.check_dropout(add, 0.3, ops.DropoutRng(4, 5), 6, torch.empty_like(add), add, (4, 5))
+    t.check_dropout(add[:, :-1], 0.3, ops.DropoutRng(4, 5), 6, torch.empty_like(add)[:, 1:], None, (4, 5))
+print("folded ok")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, NBO_GRID_X_MAX="7", PYTHONPATH=root)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=root, env=env)
+    assert r.returncode == 0 and "folded ok" in r.stdout, r.stdout[-2000:] + r.stderr[-3000:]

@@ -186,3 +186,83 @@ def test_python_arguments_are_checked():
     m = ops._matrix(torch.zeros(7, dtype=torch.float16))
     assert (m.rows, m.cols, m.dtype) == (1, 7, F16)
     assert ops._ids(torch.zeros(2, 3, dtype=torch.int32)).n == 6
+
+
+def test_rust_declarations_agree_with_the_header():
+    """integration/rust/ops.rs cannot be compiled here: the same symbols, and for every argument the
+    same kind and width."""
+    c_kind = {"double": "f64", "uint64_t": "u64", "uint32_t": "u32", "int": "int", "int32_t": "i32"}
+    r_kind = {"f64": "f64", "u64": "u64", "u32": "u32", "c_int": "int", "i32": "i32"}
+    c, rust = {}, {}
+    for name, args in re.findall(r"\bint (nbo_[a-z0-9_]+)\s*\(([^)]*)\)\s*;", _decls()):
+        c[name] = ["ptr" if "*" in a else c_kind[a.replace("const", "").split()[0]] for a in args.split(",")]
+    text = re.sub(r"//.*", "", open(os.path.join(ROOT, "integration", "rust", "ops.rs")).read())
+    for name, args in re.findall(r"pub fn (nbo_[a-z0-9_]+)\s*\(([^)]*)\)\s*->\s*c_int;", text):
+        kinds = [a.split(":", 1)[1].strip() for a in args.split(",")]
+        rust[name] = ["ptr" if k.startswith("*") else r_kind[k] for k in kinds]
+    assert c == rust and len(c) == 10
+    for c_name, r_name in (("nbo_matrix", "NboMatrix"), ("nbo_ids", "NboIds")):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (c_name, c_name), _decls(), flags=re.S).group(1)
+        want = []
+        for d in body.split(";"):
+            if d.strip():
+                ty, names = re.match(r"\s*((?:const )?\w+)\s+(.*)", d.strip(), flags=re.S).groups()
+                want += [(n.strip(" *"), "ptr" if "*" in n else c_kind[ty]) for n in names.split(",")]
+        rbody = re.search(r"pub struct %s \{(.*?)\}" % r_name, text, flags=re.S).group(1)
+        got = [(n.rstrip("_"), "ptr" if t.strip().startswith("*") else r_kind[t.strip()])
+               for n, t in re.findall(r"pub (\w+): ([^,]+)", rbody)]
+        assert got == want, (got, want)
+    for name in ("NBO_ID_I32", "NBO_ID_I64"):
+        assert int(re.search(r"\b%s = (\d+)" % name, _decls()).group(1)) == int(
+            re.search(r"pub const %s: i32 = (\d+);" % name, text).group(1))
+
+
+def test_cpp_program_is_built():
+    assert os.path.exists(os.path.join(ROOT, "tests", "cpp", "test_ops.bin")), "build it with `make -C tests/cpp`"
+
+
+class _Rng:
+    """What TrainerTail needs of a DropoutRng."""
+
+    def __init__(self, step):
+        self.at = ops.DropoutRngState(9, step)
+
+    def state(self):
+        return ops.DropoutRngState(self.at.seed, self.at.step)
+
+    def load_state(self, state):
+        self.at = ops.DropoutRngState(state.seed, state.step)
+
+    def advance(self, steps=1):
+        self.at.step = (self.at.step + steps) % (1 << 64)
+
+
+def test_trainer_tail_advances_the_generator_once_per_micro_batch():
+    from nabla_amd.checkpoint import TrainState
+    from nabla_amd.trainer import TrainerTail
+
+    class Opt:
+        def fused_step(self, *a, **k):
+            if self.fail:
+                raise RuntimeError("no")
+
+    opt = Opt()
+    opt.fail = False
+    rng = _Rng((1 << 64) - 2)
+    tail = TrainerTail(opt, []).with_rng(rng)
+    assert tail.state.rng_state == (1 << 64) - 2
+    assert tail.after_backward([]) and tail.after_backward([])
+    assert rng.at.step == 0 == tail.state.rng_state and tail.state.step == 2
+    opt.fail = True
+    with pytest.raises(RuntimeError):
+        tail.after_backward([])
+    assert rng.at.step == 1 == tail.state.rng_state and tail.state.step == 2
+    # a restored state moves the generator, before or after it is attached
+    tail.set_state(TrainState(epoch=1, step=7, grad_accum=1, rng_state=40))
+    assert rng.at == ops.DropoutRngState(9, 40)
+    other = TrainerTail(opt, [])
+    other.set_state(TrainState(rng_state=50))
+    other.with_rng(rng)
+    assert rng.at.step == 50
+    other.set_state(TrainState(rng_state=None))  # a checkpoint without one: the generator's own
+    assert rng.at.step == 50 == other.state.rng_state
