@@ -226,10 +226,10 @@ int launch_order(const nbo_ids &ids, uint64_t rows, const NboClearArgs &clear, n
     const int bits = bits_of(rows); // (the key of ids outside the table is `rows` itself)
     // 256 ranges at most, while their keys' counters fit the merge's LDS; then up to 1024
     const int shift = std::min(std::max(bits - 8, 0), (int)NBO_SPLIT_SHIFT);
-    if ((rows >> shift) + 1 <= 1ull << NBO_RADIX_BITS) {
+    if (((rows - 1) >> shift) + 1 <= 1ull << NBO_RADIX_BITS) {
         a.tiles = grid_of(ids.n, NBO_SPLIT_TILE);
         a.shift = (uint32_t)shift;
-        a.digits = (uint32_t)(rows >> shift) + 1;
+        a.digits = (uint32_t)((rows - 1) >> shift) + 1;
         a.keys_out = ws->keys[1];
         a.pos_out = ws->pos[1];
         rt.launch(K_ORDER_SPLIT, a.tiles, NBO_RADIX_BLOCK, a);
@@ -418,7 +418,7 @@ int nbo_embedding_grad(const nbo_matrix *grad_out, const nbo_ids *ids, double sc
         }
         if (ids->n <= NBO_EMBED_DIRECT_MAX) {
             a.ids = ids->data;
-            a.sum_wgs = grid_of(ids->n * a.slabs, waves_per_wg);
+            a.sum_wgs = grid_of(ids->n * a.slabs, 1);
             const uint32_t clear_wgs = accumulate ? 0 : grid_of(grad->rows, NBO_CLEAR_ROWS * waves_per_wg);
             rt.launch_folded(K_EMBED_DIRECT_BASE + pair, grid_of((uint64_t)a.sum_wgs + clear_wgs, 1), NBO_OPS_BLOCK, a);
             return;
@@ -438,7 +438,7 @@ int nbo_embedding_grad(const nbo_matrix *grad_out, const nbo_ids *ids, double sc
         a.sum_wgs = grid_of(waves, waves_per_wg);
         const uint32_t clear_wgs = a.clear.grad ? grid_of(a.clear_units.total, NBO_OPS_BLOCK) : 0;
         rt.launch_folded(K_EMBED_SUM_BASE + pair, grid_of((uint64_t)a.sum_wgs + clear_wgs, 1), NBO_OPS_BLOCK, a);
-        // (more ids than the direct form takes: there are at least five pieces)
+        // (more ids than the direct form takes: there are at least nine pieces)
         rt.launch_folded(K_EMBED_JOIN_BASE + pair, grid_of((uint64_t)(a.pieces - 1) * a.slabs, 1), NBO_OPS_BLOCK, a);
     });
 }

@@ -76,7 +76,7 @@ struct NboRngAdvanceArgs {
 #define NBO_SPLIT_TILE 1024u
 #define NBO_SPLIT_SHIFT 9u
 // Up to this many ids the gradient is one launch that needs no order.
-#define NBO_EMBED_DIRECT_MAX 256u
+#define NBO_EMBED_DIRECT_MAX 512u
 
 // Rows to clear: those of grad that no id names (grad null: none).
 #define NBO_CLEAR_ROWS 4u // per wave, where it has to find out which
@@ -120,7 +120,7 @@ struct NboEmbedGradArgs {
     uint32_t n, rows, cols;
     uint32_t units;               // per row
     uint32_t lanes;               // lanes that work on one piece: 64, or a power of two that holds `units`
-    uint32_t slabs;               // waves per piece (lanes == 64)
+    uint32_t slabs;               // waves per piece: 64 units each
     uint32_t piece, pieces;       // ids per piece, pieces
     uint32_t sum_wgs;             // workgroups that add; those behind them clear
     uint32_t accumulate;

@@ -3,6 +3,7 @@ memory system's own ceilings.
 
     python -m nabla_amd.kernel_bench [--elements 805e6] [--reps 5]
     python -m nabla_amd.kernel_bench --ceilings [--gib 2] [--reps 10]
+    python -m nabla_amd.kernel_bench --ops [--reps 30]
 
 Each entry point is timed with the library's own per-kernel HIP events on its launch stream
 (`nbo_profile_enable` / `nbo_profile_read`) and priced at its algorithmic bytes per element;
@@ -304,6 +305,90 @@ def flow_main(args) -> None:
     print(f"\nThe fused call takes {rows[1] / rows[0] * 100:.0f} % of the four calls' time.")
 
 
+def ops_main(args) -> None:
+    """The operators of nabla_ops.h (embedding lookup, its gradient, dropout) at the shapes of the
+    workloads: wall time of a call among others, and of each kernel it launches."""
+    import time
+
+    import torch
+
+    from . import _lib
+    from . import ops
+
+    _lib.init()
+    L = _lib.load()
+    dev = torch.device("cuda:0")
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(1)
+
+    def tokens(n, rows):  # log-uniform over the ranks, spread over the table
+        u = torch.rand(n, generator=gen, device=dev, dtype=torch.float64)
+        rank = ((rows + 1.0) ** u - 1).long().clamp_(0, rows - 1)
+        return (rank * 1000003 + 17) % rows
+
+    def rand(rows, cols, dtype):
+        return torch.empty(rows, cols, device=dev).normal_(generator=gen).to(dtype)
+
+    bf16, f32 = torch.bfloat16, torch.float32
+    print(f"{args.reps} calls each; GB/s over the bytes the operator cannot do without (every row named read or written once)\n")
+    print("| operator | shape | us per call | MB | GB/s | kernels (us) |")
+    print("|---|---|---|---|---|---|")
+
+    def row(name, shape, fn, nbytes, kernels):
+        for _ in range(5):
+            fn()
+        _lib.check(L.nbo_sync())
+        t0 = time.perf_counter()
+        for _ in range(args.reps):
+            fn()
+        _lib.check(L.nbo_sync())
+        us = (time.perf_counter() - t0) / args.reps * 1e6
+        _lib.check(L.nbo_profile_enable(1))
+        for _ in range(args.reps):
+            fn()
+        _lib.check(L.nbo_sync())
+        parts = []
+        for k in kernels:
+            cnt, ms = C.c_uint64(0), C.c_double(0)
+            _lib.check(L.nbo_profile_read(k.encode(), C.byref(cnt), C.byref(ms)))
+            if cnt.value:
+                parts.append(f"`{k}` {ms.value / args.reps * 1e3:.1f}")
+        _lib.check(L.nbo_profile_enable(0))
+        print(f"| {name} | {shape} | {us:.1f} | {nbytes / 1e6:.2f} | {nbytes / us / 1e3:.0f} | {', '.join(parts)} |", flush=True)
+
+    order = ["nbo_order_range", "nbo_order_split", "nbo_order_merge"]
+    for rows, cols, n, dtype, tag, gdtype, gtag in ((128256, 4096, 1, bf16, "bf16", bf16, "bf16"),
+                                                    (50257, 768, 8192, f32, "f32", f32, "f32"),
+                                                    (32000, 2048, 16384, bf16, "bf16", f32, "bf16_f32"),
+                                                    (128256, 4096, 65536, bf16, "bf16", bf16, "bf16")):
+        size, gsize = dtype.itemsize, gdtype.itemsize
+        ids = tokens(n, rows)
+        named = int(torch.unique(ids).numel())
+        shape = f"{n} of {rows} x {cols}"
+        table, out = rand(rows, cols, dtype), rand(n, cols, dtype)
+        row(f"embedding {tag}", shape, lambda: ops.embedding(table, ids, out), n * 8 + (named + n) * cols * size,
+            [f"nbo_embed_{tag}"])
+        grad = table if gdtype == dtype else rand(rows, cols, gdtype)
+        ws = ops.EmbeddingWorkspace(n, cols)
+        kernels = order + [f"nbo_embed_{k}_{gtag}" for k in ("sum", "join", "direct")]
+        for accumulate in (False, True):
+            row(f"embedding_grad {gtag}{' accumulate' if accumulate else ''}", shape,
+                lambda: ops.embedding_grad(out, ids, grad, ws, accumulate=accumulate),
+                n * 8 + n * cols * size + (2 * named if accumulate else rows) * cols * gsize, kernels)
+        del table, out, grad, ws
+        torch.cuda.empty_cache()
+    rng = ops.DropoutRng(1)
+    for rows, cols, dtype, tag in ((32, 768, bf16, "bf16"), (8192, 768, f32, "f32"), (32768, 4096, bf16, "bf16")):
+        x, r = rand(rows, cols, dtype), rand(rows, cols, dtype)
+        out = torch.empty_like(x)
+        for residual in (None, r):
+            row(f"dropout {tag}{' + residual' if residual is not None else ''}", f"{rows} x {cols}",
+                lambda: ops.dropout(x, 0.1, rng, 0, out, residual=residual),
+                x.numel() * dtype.itemsize * (2 if residual is None else 3), [f"nbo_dropout_{tag}"])
+        del x, r, out
+        torch.cuda.empty_cache()
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("--elements", type=float, default=805e6)
@@ -320,6 +405,7 @@ def main() -> None:
                          "(nbo_alloc_placed): one region against several")
     ap.add_argument("--flow", action="store_true",
                     help="a training step's tail as the reference's four calls against the one fused call")
+    ap.add_argument("--ops", action="store_true", help="the operators beside the step: embedding lookup, its gradient, dropout")
     ap.add_argument("--summarize", metavar="DIR", help="turn the rocprofv3 output under DIR into profiles/ summaries "
                                                         "(see nabla_amd/profile_summary.py) instead of measuring")
     args = ap.parse_args()
@@ -331,6 +417,10 @@ def main() -> None:
     if args.flow:
         args.reps = args.reps or 10
         flow_main(args)
+        return
+    if args.ops:
+        args.reps = args.reps or 30
+        ops_main(args)
         return
     if args.compare:
         args.reps = args.reps or 5
