@@ -157,6 +157,9 @@ uint64_t unit_elems(int a, int b) { return 16 / std::min(size_of(a), size_of(b))
 // it one id after the other).
 constexpr uint64_t SUM_WAVES = 4096;
 constexpr uint64_t PIECE_MAX = 64, PIECE_MIN = 8;
+// Most workgroups of the join, 16 for each compute unit; with more boundaries than that a workgroup looks at
+// several (1023 boundaries and 8 slabs each: 13.4 us, one to a workgroup 15.8).
+constexpr uint64_t JOIN_WGS = 4096;
 
 // lanes that work on one piece
 uint64_t piece_lanes(uint64_t units)
@@ -438,8 +441,10 @@ int nbo_embedding_grad(const nbo_matrix *grad_out, const nbo_ids *ids, double sc
         a.sum_wgs = grid_of(waves, waves_per_wg);
         const uint32_t clear_wgs = a.clear.grad ? grid_of(a.clear_units.total, NBO_OPS_BLOCK) : 0;
         rt.launch_folded(K_EMBED_SUM_BASE + pair, grid_of((uint64_t)a.sum_wgs + clear_wgs, 1), NBO_OPS_BLOCK, a);
-        // (more ids than the direct form takes: there are at least nine pieces)
-        rt.launch_folded(K_EMBED_JOIN_BASE + pair, grid_of((uint64_t)(a.pieces - 1) * a.slabs, 1), NBO_OPS_BLOCK, a);
+        // (more ids than the direct form takes are at least nine pieces)
+        const uint64_t edges = a.pieces - 1;
+        a.edges = (uint32_t)std::min<uint64_t>(64, ceil_div(edges * a.slabs, JOIN_WGS));
+        rt.launch_folded(K_EMBED_JOIN_BASE + pair, grid_of(ceil_div(edges, a.edges) * a.slabs, 1), NBO_OPS_BLOCK, a);
     });
 }
 
@@ -546,7 +551,8 @@ int nbo_dropout(const nbo_matrix *x, const nbo_matrix *residual, double p, nbo_r
         a.residual_stride = residual ? residual->stride * eb : 0;
         a.out_stride = out->stride * eb;
         a.flat = adjacent(*x) && adjacent(*out) && (!residual || adjacent(*residual)) ? 1u : 0u;
-        a.u = a.flat ? units_of(1, ceil_div(n, unit)) : units_of(x->rows, ceil_div(x->cols, unit));
+        if (a.flat) a.u.total = ceil_div(n, unit);
+        else a.u = units_of(x->rows, ceil_div(x->cols, unit));
         a.rng = rng->dev;
         const uint32_t thr = (uint32_t)std::floor(p * 65536.0 + 0.5);
         a.thr = thr;

@@ -866,7 +866,10 @@ template <typename A, int V> DEV void load_slot(const char *p, A (&x)[V])
     }
 }
 
-// One piece by `lanes` < 64 lanes, for rows of few units: several pieces to a wave.
+// One piece by `lanes` < 64 lanes, for rows of few units: several pieces to a wave.  65536 rows of 48 bf16 take
+// 13 us, the latency of 8 tokens one after the other.  (Eight tokens and their rows of the table asked for
+// together take 10, but 157 registers instead of 69, and then the clears that share this kernel are slower
+// everywhere: 128256 rows of 8 KiB 375 us instead of 282.)
 template <int ED, int EG, bool TINY> DEV void sum_narrow(const NboEmbedGradArgs &a, uint32_t wave)
 {
     enum { V = Pair<ED, EG>::V, SD = sizeof(typename El<ED>::Bits), U = 4 };
@@ -1007,66 +1010,74 @@ template <int ED, int EG, bool TINY> DEV void embed_sum_body(const NboEmbedGradA
     else sum_wide<ED, EG>(a, wave);
 }
 
-// Rows whose tokens span pieces: the workgroups of boundary k (between pieces k and k + 1), one per slab
-// of the row, finish the row that spans it and begins in piece k.  Its sums are piece k's tail and the
-// heads of the pieces behind, as many as begin with its key; the workgroup's waves -- groups of a.lanes lanes,
-// where a row has few units -- take a run of them each.  (Narrow rows are cut into many pieces: with four
-// waves on the most frequent row's 760 sums the join of 65536 rows of 48 bf16 took 20 us.)
+// Rows whose tokens span pieces.  A row that spans boundary k (between pieces k and k + 1) and begins in piece
+// k is finished by that boundary's workgroups, one per slab of the row; a workgroup looks at a.edges boundaries.
+// The row's sums are piece k's tail and the heads of the pieces behind, as many as begin with its key; the
+// workgroup's waves -- groups of a.lanes lanes, where a row has few units -- take a run of them each.
+// (65536 rows of 4096 bf16: 13-16 us, with a workgroup per boundary 16-19; of 48 bf16, whose most frequent row has
+// 760 sums: 16, with a wave for each run of them 23.  It waits for memory: boundary, row, sums, one after the other.)
 template <int ED, int EG, bool TINY> DEV void embed_join_body(const NboEmbedGradArgs &a)
 {
     enum { V = Pair<ED, EG>::V, U = 8 };
     typedef typename El<EG>::A A;
     __shared__ A part[V][NBO_OPS_BLOCK];
     const uint32_t lane = threadIdx.x & 63u, group = threadIdx.x / a.lanes, groups = NBO_OPS_BLOCK / a.lanes;
-    const uint32_t wg = folded_workgroup(), k = wg / a.slabs;
-    const uint32_t v = (wg - k * a.slabs) * 64 + threadIdx.x % a.lanes;
-    if (k + 1 >= a.pieces) return;
-    auto *keys = GLOBAL_PTR(const uint32_t, a.keys);
-    const uint64_t edge = (uint64_t)(k + 1) * a.piece;
-    // everything there is to know is asked for at once; lane j: the key that piece k + 2 + j begins with
-    auto first_of = [&](uint64_t p) { return keys[(p < a.pieces ? p : a.pieces - 1) * a.piece]; };
-    const uint32_t key = keys[edge], ahead = keys[edge - 1], earlier = keys[k > 0 ? edge - a.piece - 1 : 0];
-    uint32_t later = first_of((uint64_t)k + 2 + lane);
-    if (key >= a.rows || ahead != key) return; // no row spans this boundary
-    if (k > 0 && earlier == key) return;       // ... or it began earlier
-    uint32_t last = k + 1; // the last piece that begins with this row (its boundary is inside the row)
-    for (;;) {
-        const uint64_t m = ~__builtin_amdgcn_ballot_w64((uint64_t)last + 1 + lane < a.pieces && later == key);
-        const uint32_t c = m ? (uint32_t)__builtin_ctzll(m) : 64u;
-        last += c;
-        if (c < 64) break;
-        later = first_of((uint64_t)last + 1 + lane);
-    }
-    const uint32_t total = last - k, per = (total + groups - 1) / groups;
+    const uint32_t wg = folded_workgroup(), k0 = wg / a.slabs * a.edges;
+    const uint32_t v = wg % a.slabs * 64 + threadIdx.x % a.lanes;
     const Span s = unit_span<V>(v < a.units ? v : a.units - 1, a.cols);
-    Unit<EG, V> g;
-    if (a.accumulate) g.template load<TINY, false>(grad_at<EG>(a, key, s), s.n);
-    A acc[V];
+    auto *keys = GLOBAL_PTR(const uint32_t, a.keys);
+    // lane j looks at boundary k0 + j
+    const uint32_t mine = k0 + lane;
+    const bool edge = lane < a.edges && mine + 1 < a.pieces;
+    const uint64_t at = edge ? (uint64_t)(mine + 1) * a.piece : a.piece; // (there are at least two pieces)
+    const uint32_t key_at = keys[at], ahead = keys[at - 1], earlier = keys[at > a.piece ? at - a.piece - 1 : 0];
+    uint64_t todo = __builtin_amdgcn_ballot_w64(edge && key_at < a.rows && ahead == key_at && (mine == 0 || earlier != key_at));
+    auto first_of = [&](uint64_t p) { return keys[(p < a.pieces ? p : a.pieces - 1) * a.piece]; };
+    for (; todo; todo &= todo - 1) {
+        const uint32_t k = k0 + __builtin_ctzll(todo), key = __builtin_amdgcn_readlane(key_at, __builtin_ctzll(todo));
+        Unit<EG, V> g;
+        if (a.accumulate) g.template load<TINY, false>(grad_at<EG>(a, key, s), s.n);
+        // the last piece that begins with this row (its boundary is inside the row): the next 64 pieces looked at
+        // one each, then, the order being sorted, 64 evenly spaced ones of what is left, as often as it takes
+        uint32_t last = k + 1, end = a.pieces, step = 1;
+        do {
+            const uint64_t p = (uint64_t)last + (uint64_t)(lane + 1) * step;
+            const uint32_t later = first_of(p);
+            const uint64_t m = ~__builtin_amdgcn_ballot_w64(p < end && later == key);
+            const uint32_t c = m ? (uint32_t)__builtin_ctzll(m) : 64u;
+            last += c * step;
+            if (c < 64 && end - last > step) end = last + step;
+            step = (end - last + 63) / 64;
+        } while (end - last > 1);
+        const uint32_t total = last - k, per = (total + groups - 1) / groups;
+        A acc[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) acc[j] = (A)0;
-    if (v < a.units) {
-        if (group == 0) load_slot<A, V>(slot_at<A, V>(a, k, SLOT_TAIL, v), acc);
-        const uint32_t lo = group * per, hi = lo + per < total ? lo + per : total;
-        for (uint32_t i = lo; i < hi; i += U) {
-            A x[U][V];
+        for (int j = 0; j < V; j++) acc[j] = (A)0;
+        if (v < a.units) {
+            if (group == 0) load_slot<A, V>(slot_at<A, V>(a, k, SLOT_TAIL, v), acc);
+            const uint32_t lo = group * per, hi = lo + per < total ? lo + per : total;
+            for (uint32_t i = lo; i < hi; i += U) {
+                A x[U][V];
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (i + u < hi) load_slot<A, V>(slot_at<A, V>(a, k + 1 + i + u, SLOT_HEAD, v), x[u]);
+                for (int u = 0; u < U; u++)
+                    if (i + u < hi) load_slot<A, V>(slot_at<A, V>(a, k + 1 + i + u, SLOT_HEAD, v), x[u]);
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (i + u < hi)
+                for (int u = 0; u < U; u++)
+                    if (i + u < hi)
 #pragma unroll
-                    for (int j = 0; j < V; j++) acc[j] += x[u][j];
+                        for (int j = 0; j < V; j++) acc[j] += x[u][j];
+            }
         }
-    }
+        __syncthreads(); // (the boundary before has been read)
 #pragma unroll
-    for (int j = 0; j < V; j++) part[j][threadIdx.x] = acc[j];
-    __syncthreads();
-    if (group == 0 && v < a.units) {
-        for (uint32_t q = 1; q < groups; q++)
+        for (int j = 0; j < V; j++) part[j][threadIdx.x] = acc[j];
+        __syncthreads();
+        if (group == 0 && v < a.units) {
+            for (uint32_t q = 1; q < groups; q++)
 #pragma unroll
-            for (int j = 0; j < V; j++) acc[j] += part[j][q * a.lanes + threadIdx.x];
-        finish_row<EG, V>(a, key, s, g, acc);
+                for (int j = 0; j < V; j++) acc[j] += part[j][q * a.lanes + threadIdx.x];
+            finish_row<EG, V>(a, key, s, g, acc);
+        }
     }
 }
 

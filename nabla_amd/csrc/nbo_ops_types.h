@@ -122,6 +122,7 @@ struct NboEmbedGradArgs {
     uint32_t lanes;               // lanes that work on one piece: 64, or a power of two that holds `units`
     uint32_t slabs;               // waves per piece: 64 units each
     uint32_t piece, pieces;       // ids per piece, pieces
+    uint32_t edges;               // boundaries between pieces per workgroup of the join, at most 64
     uint32_t sum_wgs;             // workgroups that add; those behind them clear
     uint32_t accumulate;
     uint32_t ids64;

@@ -441,6 +441,22 @@ def test_offsets_beyond_32_bits(gpu):
     assert torch.equal(table.reshape(-1)[first:].float(), keep.float() * 2)
 
 
+def test_dropout_of_more_units_than_32_bits(gpu):
+    """2^32 units and a few: f64 elements two to a unit, 64 GiB in one run, in place."""
+    rows, cols = (1 << 23) + 1, 1024
+    n = rows * cols
+    if torch.cuda.mem_get_info(DEV)[0] < n * 8 + (1 << 30):
+        pytest.skip("needs 65 GiB of free device memory")
+    x = torch.ones(rows, cols, device=DEV, dtype=torch.float64)
+    ops.dropout(x, 0.5, ops.DropoutRng(21, 2), 1, x)
+    x = x.reshape(-1)
+    first = n - 4096
+    assert torch.equal(x[first:], kept(n - first, 21, 2, 1, 0.5, first)[0].double() * 2)
+    assert torch.equal(x[:4096], kept(4096, 21, 2, 1, 0.5)[0].double() * 2)
+    del x
+    torch.cuda.empty_cache()
+
+
 # ---- together, as a training step uses them ---------------------------------------------------
 
 class _InputBlock:
