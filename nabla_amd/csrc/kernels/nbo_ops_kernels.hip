@@ -678,6 +678,9 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
     const uint32_t per = (a.tiles + WAVES - 1) / WAVES;
     const uint32_t from = wave * per, to = from + per < a.tiles ? from + per : a.tiles;
     auto *ends = GLOBAL_PTR(const uint32_t, a.hist) + (uint64_t)a.digits * a.tiles; // ids that count, per tile
+    // (where the wave's first segments lie is asked for together with the sums' terms)
+    auto tile_at = [&](uint32_t t0) { return t0 + (lane & 3u) < a.tiles ? t0 + (lane & 3u) : a.tiles - 1; };
+    const uint32_t first_start = h[tile_at(from)], first_end = h[a.tiles + tile_at(from)];
     uint32_t below = 0, valid = 0;
     for (uint32_t t = threadIdx.x; t < a.tiles; t += NBO_RANGE_BLOCK) {
         below += h[t];
@@ -691,9 +694,7 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
     // The wave's tiles in order, four at a time: the first 64 ids of the range in each of the four are asked
     // for together, with their places, and kept where there is but one such group (up to 64 tiles)
     uint32_t at[U], len[U], key[U], pos[U];
-    auto fetch = [&](uint32_t t0) {
-        const uint32_t tl = t0 + (lane & 3u) < a.tiles ? t0 + (lane & 3u) : a.tiles - 1;
-        const uint32_t start = h[tl], end = h[a.tiles + tl];
+    auto fetch = [&](uint32_t t0, uint32_t start, uint32_t end) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const uint32_t s = __builtin_amdgcn_readlane(start, u);
@@ -729,10 +730,10 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
                 if (o + j * 64 < n) each(k[j], p[j], __builtin_amdgcn_ballot_w64(o + j * 64 + lane < n));
         }
     };
-    if (from < to) fetch(from);
+    if (from < to) fetch(from, first_start, first_end);
     __syncthreads();
     for (uint32_t t0 = from; t0 < to; t0 += U) {
-        if (t0 > from) fetch(t0);
+        if (t0 > from) fetch(t0, h[tile_at(t0)], h[a.tiles + tile_at(t0)]);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (len[u] == 0) continue;
@@ -742,7 +743,7 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
     }
     starts_of_keys<WAVES>(a, lo, count, range, below, wsum, wbelow);
     for (uint32_t t0 = from; t0 < to; t0 += U) {
-        if (per > U) fetch(t0);
+        if (per > U) fetch(t0, h[tile_at(t0)], h[a.tiles + tile_at(t0)]);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (len[u] == 0) continue;
@@ -1026,29 +1027,32 @@ template <int ED, int EG, bool TINY> DEV void embed_join_body(const NboEmbedGrad
     const uint32_t v = wg % a.slabs * 64 + threadIdx.x % a.lanes;
     const Span s = unit_span<V>(v < a.units ? v : a.units - 1, a.cols);
     auto *keys = GLOBAL_PTR(const uint32_t, a.keys);
-    // lane j looks at boundary k0 + j
+    // lane j looks at boundary k0 + j, past the workgroup's own ones for where their rows end
     const uint32_t mine = k0 + lane;
-    const bool edge = lane < a.edges && mine + 1 < a.pieces;
+    const bool edge = mine + 1 < a.pieces;
     const uint64_t at = edge ? (uint64_t)(mine + 1) * a.piece : a.piece; // (there are at least two pieces)
     const uint32_t key_at = keys[at], ahead = keys[at - 1], earlier = keys[at > a.piece ? at - a.piece - 1 : 0];
-    uint64_t todo = __builtin_amdgcn_ballot_w64(edge && key_at < a.rows && ahead == key_at && (mine == 0 || earlier != key_at));
+    uint64_t todo = __builtin_amdgcn_ballot_w64(edge && lane < a.edges && key_at < a.rows && ahead == key_at &&
+                                                (mine == 0 || earlier != key_at));
     auto first_of = [&](uint64_t p) { return keys[(p < a.pieces ? p : a.pieces - 1) * a.piece]; };
     for (; todo; todo &= todo - 1) {
-        const uint32_t k = k0 + __builtin_ctzll(todo), key = __builtin_amdgcn_readlane(key_at, __builtin_ctzll(todo));
+        const uint32_t j = __builtin_ctzll(todo), k = k0 + j, key = __builtin_amdgcn_readlane(key_at, j);
         Unit<EG, V> g;
         if (a.accumulate) g.template load<TINY, false>(grad_at<EG>(a, key, s), s.n);
-        // the last piece that begins with this row (its boundary is inside the row): the next 64 pieces looked at
-        // one each, then, the order being sorted, 64 evenly spaced ones of what is left, as often as it takes
-        uint32_t last = k + 1, end = a.pieces, step = 1;
-        do {
+        // the last piece that begins with this row (its boundary is inside the row): as far as the lanes have
+        // looked, then, the order being sorted, among 64 evenly spaced pieces of what is left, as often as it takes
+        const uint64_t same = __builtin_amdgcn_ballot_w64(edge && key_at == key) >> j; // (bit 0 is this boundary)
+        const uint32_t seen = ~same ? (uint32_t)__builtin_ctzll(~same) : 64u;
+        uint32_t last = k + seen;
+        for (uint32_t end = j + seen < 64 ? last + 1 : a.pieces; end - last > 1;) {
+            const uint32_t step = (end - last + 63) / 64;
             const uint64_t p = (uint64_t)last + (uint64_t)(lane + 1) * step;
             const uint32_t later = first_of(p);
-            const uint64_t m = ~__builtin_amdgcn_ballot_w64(p < end && later == key);
-            const uint32_t c = m ? (uint32_t)__builtin_ctzll(m) : 64u;
+            const uint64_t m = __builtin_amdgcn_ballot_w64(p < end && later == key); // (not all: p reaches end)
+            const uint32_t c = (uint32_t)__builtin_ctzll(~m);
             last += c * step;
-            if (c < 64 && end - last > step) end = last + step;
-            step = (end - last + 63) / 64;
-        } while (end - last > 1);
+            if (end - last > step) end = last + step;
+        }
         const uint32_t total = last - k, per = (total + groups - 1) / groups;
         A acc[V];
 #pragma unroll
