@@ -196,43 +196,47 @@ int bits_of(uint64_t x)
     return b;
 }
 
-// Order by ranges (nbo_order_range): keys per workgroup, or 0 where other launches are taken.  One workgroup
-// for each of the 256 compute units, or as many as the table needs.
-uint32_t order_range(uint64_t n, uint64_t rows)
+// Into how many ranges, as a power of two, the rows are dealt out: one for each of the 256 compute units, or
+// as many as leave at most `keys` to each.
+uint32_t range_shift(uint64_t rows, uint64_t keys)
 {
-    if (n > NBO_RANGE_IDS || rows > NBO_NAMED_ROWS) return 0;
-    return (uint32_t)std::min<uint64_t>(ceil_div(rows + 1, 256), NBO_RANGE_KEYS);
+    uint32_t shift = 8;
+    while (((rows - 1) >> shift) + 1 > keys) shift++;
+    return shift;
 }
 
-// The ids in table order into (keys, pos) of the workspace; returns which of the two buffers.  With rows to
-// clear, *named says which rows have ids, or is null and they have been cleared.
-int launch_order(const nbo_ids &ids, uint64_t rows, const NboClearArgs &clear, nbo_embedding_ws *ws, const uint8_t **named)
+// The tokens ordered by rows into (keys, pos) of the workspace; returns which of the two buffers.  With rows to
+// clear, g.named says which rows have ids, or is null and they have been cleared.
+int launch_order(const nbo_ids &ids, uint64_t rows, nbo_embedding_ws *ws, NboEmbedGradArgs &g)
 {
     Runtime &rt = Runtime::get();
     NboOrderArgs a = {};
-    a.clear = clear;
-    a.named = clear.grad ? ws->named : nullptr;
-    *named = a.named;
+    a.clear = g.clear;
     a.ids = ids.data;
     a.ids64 = ids.type == NBO_ID_I64;
     a.n = (uint32_t)ids.n;
     a.rows = (uint32_t)rows;
     a.hist = ws->hist;
     a.totals = ws->totals;
-    a.range = order_range(ids.n, rows);
-    if (a.range) {
+    auto deal_out = [&](uint32_t shift) {
+        a.shift = shift;
+        a.digits = (uint32_t)std::min<uint64_t>(rows, 1ull << shift);
+        a.range = (uint32_t)((rows - 1) >> shift) + 1;
+        a.named = g.clear.grad ? ws->named : nullptr;
+        g.named = a.named;
+        g.named_shift = a.shift;
+        g.named_range = a.range;
+    };
+    if (ids.n <= NBO_RANGE_IDS && rows <= NBO_NAMED_ROWS) {
+        deal_out(range_shift(rows, NBO_RANGE_KEYS));
         a.keys_out = ws->keys[0];
         a.pos_out = ws->pos[0];
-        rt.launch(K_ORDER_RANGE, grid_of(rows + 1, a.range), NBO_RANGE_BLOCK, a, NBO_RANGE_BLOCK / 64 * 4 * a.range);
+        rt.launch(K_ORDER_RANGE, a.digits, NBO_RANGE_BLOCK, a, NBO_RANGE_BLOCK / 64 * 4 * a.range);
         return 0;
     }
-    const int bits = bits_of(rows); // (the key of ids outside the table is `rows` itself)
-    // 256 ranges at most, while their keys' counters fit the merge's LDS; then up to 1024
-    const int shift = std::min(std::max(bits - 8, 0), (int)NBO_SPLIT_SHIFT);
-    if (((rows - 1) >> shift) + 1 <= 1ull << NBO_RADIX_BITS) {
+    if (rows <= (uint64_t)NBO_SPLIT_KEYS << NBO_RADIX_BITS) {
+        deal_out(range_shift(rows, NBO_SPLIT_KEYS));
         a.tiles = grid_of(ids.n, NBO_SPLIT_TILE);
-        a.shift = (uint32_t)shift;
-        a.digits = (uint32_t)((rows - 1) >> shift) + 1;
         a.keys_out = ws->keys[1];
         a.pos_out = ws->pos[1];
         rt.launch(K_ORDER_SPLIT, a.tiles, NBO_RADIX_BLOCK, a);
@@ -243,8 +247,7 @@ int launch_order(const nbo_ids &ids, uint64_t rows, const NboClearArgs &clear, n
         rt.launch(K_ORDER_MERGE, a.digits, NBO_RANGE_BLOCK, a);
         return 0;
     }
-    a.named = nullptr;
-    *named = nullptr;
+    const int bits = bits_of(rows); // (the key of ids outside the table is `rows` itself)
     const int passes = (bits + NBO_RADIX_BITS - 1) / NBO_RADIX_BITS;
     const int per = (bits + passes - 1) / passes;
     a.tiles = grid_of(ids.n, NBO_RADIX_TILE);
@@ -261,7 +264,7 @@ int launch_order(const nbo_ids &ids, uint64_t rows, const NboClearArgs &clear, n
         rt.launch(K_ORDER_SCAN, a.digits, 64, a);
         rt.launch(K_ORDER_SCATTER, a.tiles, NBO_RADIX_BLOCK, a);
     }
-    if (clear.grad) {
+    if (g.clear.grad) {
         a.keys_in = ws->keys[to];
         rt.launch_folded(K_ORDER_CLEAR, grid_of(rows, NBO_CLEAR_ROWS * NBO_OPS_BLOCK / 64), NBO_OPS_BLOCK, a);
     }
@@ -432,7 +435,7 @@ int nbo_embedding_grad(const nbo_matrix *grad_out, const nbo_ids *ids, double sc
         // (twice, of sums of 4 or 8 bytes)
         const uint64_t need = 2ull * a.pieces * a.units * unit * (grad->dtype == NBO_DT_F64 ? 8 : 4);
         require(need <= ws->partial_bytes, NBO_ERR_TOO_LARGE, "internal: the workspace's partial sums are too small");
-        const int order = launch_order(*ids, grad->rows, a.clear, ws, &a.named);
+        const int order = launch_order(*ids, grad->rows, ws, a);
         if (!a.named) a.clear.grad = nullptr;
         a.keys = ws->keys[order];
         a.pos = ws->pos[order];

@@ -2,7 +2,7 @@
 // and dropout from a counter-based generator.  A code object of its own beside the optimizer's.
 //
 //   nbo_embed_*        out[t] = add[t] + scale * table[ids[t]]
-//   nbo_order_range    the ids in table order, in one launch (up to 8192 ids)
+//   nbo_order_range    the tokens ordered by rows, in one launch (up to 8192 ids)
 //   nbo_order_split / _merge             ... in two (more ids)
 //   nbo_order_hist / _scan / _scatter    ... by radix passes (tables of more than half a million rows)
 //   nbo_order_clear    zeros in the rows no id names, behind the radix passes
@@ -185,15 +185,19 @@ DEV UnitBase unit_base(const NboUnits &u, uint64_t base)
     b.first = (uint32_t)(base - b.row * u.per_row);
     return b;
 }
-DEV void unit_at(const NboUnits &u, const UnitBase &b, uint32_t x, uint64_t *row, uint32_t *v)
+DEV void unit_from(const NboUnits &u, const UnitBase &b, uint32_t x, uint32_t *rows_on, uint32_t *v)
 {
     const uint32_t y = b.first + x;
-    uint32_t q;
-    if (u.per_row == 1) q = y;
-    else if (u.per_row < 1024) q = __umulhi(y, u.m32);
-    else q = y >= u.per_row ? 1u : 0u;
-    *row = b.row + q;
-    *v = y - q * u.per_row;
+    if (u.per_row == 1) *rows_on = y;
+    else if (u.per_row < 1024) *rows_on = __umulhi(y, u.m32);
+    else *rows_on = y >= u.per_row ? 1u : 0u;
+    *v = y - *rows_on * u.per_row;
+}
+DEV void unit_at(const NboUnits &u, const UnitBase &b, uint32_t x, uint64_t *row, uint32_t *v)
+{
+    uint32_t on;
+    unit_from(u, b, x, &on, v);
+    *row = b.row + on;
 }
 
 // The ids of U tokens as rows of the table, `rows` for one outside it.  (All loads first, then the keys: a
@@ -300,10 +304,16 @@ DEV uint32_t wave_scan(uint32_t x)
 }
 
 // ---------------------------------------------------------------------------------
-// Table order in one launch: every workgroup owns a range of keys, reads all ids and puts those of its
-// range to their places.  Nothing passes between workgroups: how many ids come before the range is
-// counted on the way.  Within the range an id's place is its key's start, the ids of that key which
-// earlier waves hold (each wave has a run of the ids), and those its own wave has seen.
+// The order.  All that the sums need is that the tokens of one row are adjacent and in their own order, so
+// rows are dealt out to 2^shift ranges, row v to range v % 2^shift: ids that are close to one another (a
+// vocabulary sorted by frequency, positions) are spread over all ranges.  Ranges come in order, within a range the
+// rows, within a row its tokens; padding takes no part, and the places behind the last token hold its key.
+// (With ranges of adjacent rows the merge of 65536 ids, log-uniform over 131072 rows, took 57 us instead of NEW1.)
+//
+// In one launch: every workgroup owns a range, reads all ids and puts those of its range to their places.
+// Nothing passes between workgroups: how many ids come before the range is counted on the way.  Within the
+// range an id's place is its key's start, the ids of that key which earlier waves hold (each wave has a run of
+// the ids), and those its own wave has seen.
 
 // For a block of 64 ids of which the lanes in `left` (not empty) count: adds to mine[r] how many lanes hold
 // each r.  The lanes that hold what the first one holds are counted as one: an addition to one LDS word takes
@@ -354,33 +364,42 @@ DEV uint32_t place_keys(uint32_t *mine, uint32_t r, uint64_t left, uint32_t bits
     return on ? start + ahead : at;
 }
 
-// count[WAVES][range], each wave's number of ids of each key, becomes where the wave's first one goes:
-// behind the `below` (summed over the waves) ids before the range, the smaller keys, the waves before.
-// One thread per key; range is at most the workgroup's size.  Notes in a.named which rows of the table have
-// ids (lo: the range's first key).
-template <int WAVES> DEV void starts_of_keys(const NboOrderArgs &a, uint32_t lo, uint32_t *count, uint32_t range,
-                                             uint32_t below, uint32_t (&wsum)[WAVES], uint32_t (&wbelow)[WAVES])
+// a workgroup's sum: one term per wave, to be added up behind a barrier
+template <int WAVES> DEV void leave_sum(uint32_t x, uint32_t (&terms)[WAVES])
 {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int s = 32; s >= 1; s /= 2) below += __shfl_xor(below, s);
-    if (lane == 0) wbelow[wave] = below;
+    for (int s = 32; s >= 1; s /= 2) x += __shfl_xor(x, s);
+    if ((threadIdx.x & 63u) == 0) terms[threadIdx.x >> 6] = x;
+}
+template <int WAVES> DEV uint32_t total_of(const uint32_t (&terms)[WAVES])
+{
+    uint32_t x = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) x += terms[w];
+    return x;
+}
+
+// count[WAVES][range], each wave's number of ids of each key, becomes where the wave's first one goes:
+// behind the ids of the ranges before (wbelow: one term per wave), the smaller keys, the waves before.
+// One thread per key; range is at most the workgroup's size.  Notes in a.named which rows of the table have
+// ids, range by range.
+template <int WAVES> DEV void starts_of_keys(const NboOrderArgs &a, uint32_t *count, uint32_t (&wsum)[WAVES],
+                                             const uint32_t (&wbelow)[WAVES])
+{
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, range = a.range;
     __syncthreads();
     uint32_t c[WAVES], total = 0;
     if (threadIdx.x < range)
 #pragma unroll
         for (int w = 0; w < WAVES; w++) total += c[w] = count[w * range + threadIdx.x];
-    if (a.named && threadIdx.x < range && lo + threadIdx.x < a.rows)
-        GLOBAL_PTR(uint8_t, a.named)[lo + threadIdx.x] = total > 0;
+    if (a.named && threadIdx.x < range) GLOBAL_PTR(uint8_t, a.named)[(uint64_t)blockIdx.x * range + threadIdx.x] = total > 0;
     const uint32_t up = wave_scan(total);
     if (lane == 63) wsum[wave] = up;
     __syncthreads();
-    uint32_t at = up - total;
+    uint32_t at = up - total + total_of<WAVES>(wbelow);
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) {
-        at += wbelow[w];
+    for (int w = 0; w < WAVES; w++)
         if ((uint32_t)w < wave) at += wsum[w];
-    }
     if (threadIdx.x < range)
 #pragma unroll
         for (int w = 0; w < WAVES; w++) {
@@ -388,6 +407,15 @@ template <int WAVES> DEV void starts_of_keys(const NboOrderArgs &a, uint32_t lo,
             at += c[w];
         }
     __syncthreads();
+}
+
+// the padding's key behind the last of the `valid` ids, workgroup wg's share of wgs
+DEV void fill_padding(const NboOrderArgs &a, uint32_t valid, uint32_t wg, uint32_t wgs)
+{
+    for (uint64_t i = (uint64_t)valid + wg * NBO_RANGE_BLOCK + threadIdx.x; i < a.n; i += wgs * NBO_RANGE_BLOCK) {
+        GLOBAL_PTR(uint32_t, a.keys_out)[i] = a.rows;
+        GLOBAL_PTR(uint32_t, a.pos_out)[i] = 0;
+    }
 }
 
 // Zeros in `bytes` bytes (an even number) at an even address, by a whole wave: two bytes at a time up to
@@ -426,7 +454,8 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_range(co
     __shared__ uint32_t wsum[WAVES], wbelow[WAVES];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t blocks = (a.n + 63) / 64, per = (blocks + WAVES - 1) / WAVES; // blocks of 64 ids per wave, at most U
-    const uint32_t lo = blockIdx.x * a.range, first = wave * per * 64 + lane;
+    const uint32_t first = wave * per * 64 + lane, mask = (1u << a.shift) - 1;
+    const uint32_t end = (wave + 1) * per * 64 < a.n ? (wave + 1) * per * 64 : a.n; // of the wave's run
     uint64_t t[U];
     uint32_t key[U];
 #pragma unroll
@@ -438,27 +467,29 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_range(co
     for (uint32_t i = threadIdx.x; i < WAVES * a.range; i += NBO_RANGE_BLOCK) count[i] = 0;
     __syncthreads();
     uint32_t *mine = count + wave * a.range;
-    uint32_t below = 0;
-    uint64_t in[U]; // the lanes whose ids are in the range
+    uint32_t below = 0; // the wave's ids of the ranges before
+    uint64_t in[U];     // the lanes whose ids are in the range
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const bool on = (uint32_t)u < per && first + u * 64 < a.n;
-        below += on && key[u] < lo;
-        key[u] -= lo;
-        in[u] = __builtin_amdgcn_ballot_w64(on && key[u] < a.range);
+        const uint64_t takes_part = __builtin_amdgcn_ballot_w64(first + u * 64 < end) & __builtin_amdgcn_ballot_w64(key[u] < a.rows);
+        below += (uint32_t)__popcll(takes_part & __builtin_amdgcn_ballot_w64((key[u] & mask) < blockIdx.x));
+        in[u] = takes_part & __builtin_amdgcn_ballot_w64((key[u] & mask) == blockIdx.x);
+        key[u] >>= a.shift;
         if (in[u]) count_keys(mine, key[u], in[u]);
     }
-    starts_of_keys<WAVES>(a, lo, count, a.range, below, wsum, wbelow);
-    const uint32_t bits = 32 - __builtin_clz(a.range | 1);
+    if (lane == 0) wbelow[wave] = below;
+    starts_of_keys<WAVES>(a, count, wsum, wbelow);
+    const uint32_t bits = 32 - __builtin_clz((a.range - 1) | 1);
 #pragma unroll
     for (int u = 0; u < U; u++) {
         if (!in[u]) continue;
         const uint32_t at = place_keys(mine, key[u], in[u], bits);
         if (in[u] >> lane & 1) {
-            GLOBAL_PTR(uint32_t, a.keys_out)[at] = key[u] + lo;
+            GLOBAL_PTR(uint32_t, a.keys_out)[at] = key[u] << a.shift | blockIdx.x;
             GLOBAL_PTR(uint32_t, a.pos_out)[at] = first + u * 64;
         }
     }
+    if (blockIdx.x == gridDim.x - 1) fill_padding(a, total_of<WAVES>(wbelow) + total_of<WAVES>(wsum), 0, 1);
 }
 
 // ---------------------------------------------------------------------------------
@@ -601,10 +632,9 @@ extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_scatter(
 }
 
 // ---------------------------------------------------------------------------------
-// Table order in two launches: every tile puts its ids in the order of the keys' high bits, in place,
-// and notes where each of these ranges starts; then one workgroup per range collects it from all tiles
-// and orders it as nbo_order_range does.  What lies before the range is the sum of the tiles' starts.
-// Padding takes no part; the places behind the last id get its key, a share from every workgroup.
+// The same order in two launches: every tile puts its ids in the order of the ranges, in place, and notes
+// where each range starts; then one workgroup per range collects it from all tiles and orders it as
+// nbo_order_range does.  What lies before the range is the sum of the tiles' starts.
 extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_split(const NboOrderArgs a)
 {
     enum { WAVES = NBO_RADIX_BLOCK / 64, ROWS = NBO_SPLIT_TILE / NBO_RADIX_BLOCK };
@@ -627,7 +657,7 @@ extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_split(co
 #pragma unroll
     for (int r = 0; r < ROWS; r++) {
         on[r] = on[r] && key[r] < a.rows; // padding is left out
-        digit[r] = on[r] ? key[r] >> a.shift : 0;
+        digit[r] = on[r] ? key[r] & ((1u << a.shift) - 1) : 0;
     }
     __syncthreads();
     rank_digits<ROWS>(count[wave], digit, on, a.digits, rank);
@@ -668,10 +698,10 @@ extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_split(co
 extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(const NboOrderArgs a)
 {
     enum { WAVES = NBO_RANGE_BLOCK / 64, U = 4 };
-    __shared__ uint32_t count[WAVES << NBO_SPLIT_SHIFT];
+    __shared__ uint32_t count[WAVES * NBO_SPLIT_KEYS];
     __shared__ uint32_t wsum[WAVES], wbelow[WAVES], wvalid[WAVES];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
-    const uint32_t range = 1u << a.shift, lo = blockIdx.x << a.shift;
+    const uint32_t bits = 32 - __builtin_clz((a.range - 1) | 1);
     auto *h = GLOBAL_PTR(const uint32_t, a.hist) + (uint64_t)blockIdx.x * a.tiles;
     auto *keys = GLOBAL_PTR(const uint32_t, a.keys_in);
     auto *poss = GLOBAL_PTR(const uint32_t, a.pos_in);
@@ -686,11 +716,10 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
         below += h[t];
         valid += ends[t];
     }
-    for (uint32_t i = threadIdx.x; i < WAVES * range; i += NBO_RANGE_BLOCK) count[i] = 0;
-    uint32_t *mine = count + wave * range;
-#pragma unroll
-    for (int s = 32; s >= 1; s /= 2) valid += __shfl_xor(valid, s);
-    if (lane == 0) wvalid[wave] = valid;
+    for (uint32_t i = threadIdx.x; i < WAVES * a.range; i += NBO_RANGE_BLOCK) count[i] = 0;
+    uint32_t *mine = count + wave * a.range;
+    leave_sum<WAVES>(valid, wvalid);
+    leave_sum<WAVES>(below, wbelow);
     // The wave's tiles in order, four at a time: the first 64 ids of the range in each of the four are asked
     // for together, with their places, and kept where there is but one such group (up to 64 tiles)
     uint32_t at[U], len[U], key[U], pos[U];
@@ -704,25 +733,25 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
 #pragma unroll
         for (int u = 0; u < U; u++) { // (behind the segment: its first id again, or the last of all)
             const uint32_t p = at[u] + (lane < len[u] ? lane : 0), q = p < a.n ? p : a.n - 1;
-            key[u] = keys[q] - lo;
+            key[u] = keys[q] >> a.shift;
             pos[u] = poss[q];
         }
     };
     auto place = [&](uint32_t r, uint32_t p, uint64_t in) {
-        const uint32_t to_at = place_keys(mine, r, in, a.shift);
+        const uint32_t to_at = place_keys(mine, r, in, bits);
         if (in >> lane & 1) {
-            GLOBAL_PTR(uint32_t, a.keys_out)[to_at] = r + lo;
+            GLOBAL_PTR(uint32_t, a.keys_out)[to_at] = r << a.shift | blockIdx.x;
             GLOBAL_PTR(uint32_t, a.pos_out)[to_at] = p;
         }
     };
-    // what a segment has behind its first 64 (a hot row, padding), again four blocks at a time
+    // what a segment has behind its first 64 (a hot row), again four blocks at a time
     auto behind = [&](uint32_t first, uint32_t n, auto &&each) {
         for (uint32_t o = 64; o < n; o += 64 * U) {
             uint32_t k[U], p[U];
 #pragma unroll
             for (int j = 0; j < U; j++) {
                 const uint32_t q = first + (o + j * 64 + lane < n ? o + j * 64 + lane : 0);
-                k[j] = keys[q] - lo;
+                k[j] = keys[q] >> a.shift;
                 p[j] = poss[q];
             }
 #pragma unroll
@@ -741,7 +770,7 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
             behind(at[u], len[u], [&](uint32_t r, uint32_t, uint64_t in) { count_keys(mine, r, in); });
         }
     }
-    starts_of_keys<WAVES>(a, lo, count, range, below, wsum, wbelow);
+    starts_of_keys<WAVES>(a, count, wsum, wbelow);
     for (uint32_t t0 = from; t0 < to; t0 += U) {
         if (per > U) fetch(t0, h[tile_at(t0)], h[a.tiles + tile_at(t0)]);
 #pragma unroll
@@ -751,13 +780,7 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
             behind(at[u], len[u], place);
         }
     }
-    valid = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) valid += wvalid[w];
-    for (uint64_t i = (uint64_t)valid + blockIdx.x * NBO_RANGE_BLOCK + threadIdx.x; i < a.n; i += a.digits * NBO_RANGE_BLOCK) {
-        GLOBAL_PTR(uint32_t, a.keys_out)[i] = a.rows;
-        GLOBAL_PTR(uint32_t, a.pos_out)[i] = 0;
-    }
+    fill_padding(a, total_of<WAVES>(wvalid), blockIdx.x, a.digits);
 }
 
 // First place in keys[lo .. hi) whose key is not below `key`
@@ -986,16 +1009,20 @@ DEV void clear_unnamed(const NboEmbedGradArgs &a, uint32_t wg)
 {
     const uint64_t base = (uint64_t)wg * NBO_OPS_BLOCK;
     if (base + threadIdx.x >= a.clear_units.total) return;
-    uint64_t row;
-    uint32_t v;
-    unit_at(a.clear_units, unit_base(a.clear_units, base), threadIdx.x, &row, &v);
-    if (GLOBAL_PTR(const uint8_t, a.named)[row]) return;
-    char *p = (char *)a.clear.grad + row * a.clear.grad_stride;
-    if (a.clear.row_bytes >= 16) { // (a row's last 16 bytes end with the row)
-        const uint64_t o = (uint64_t)v * 16 + 16 <= a.clear.row_bytes ? (uint64_t)v * 16 : a.clear.row_bytes - 16;
-        __builtin_nontemporal_store((u32x4_e)0, GLOBAL_PTR(u32x4_e, p + o));
+    const UnitBase b = unit_base(a.clear_units, base);
+    uint32_t on, v;
+    unit_from(a.clear_units, b, threadIdx.x, &on, &v);
+    const uint32_t row = (uint32_t)b.row + on, bytes = (uint32_t)a.clear.row_bytes;
+    if (GLOBAL_PTR(const uint8_t, a.named)[(row & ((1u << a.named_shift) - 1)) * a.named_range + (row >> a.named_shift)]) return;
+    if (bytes % 16 == 0 && a.clear.grad_stride == bytes) { // units follow one another: few instructions per store
+        __builtin_nontemporal_store((u32x4_e)0, GLOBAL_PTR(u32x4_e, (char *)a.clear.grad + base * 16 + threadIdx.x * 16));
+        return;
+    }
+    char *p = (char *)a.clear.grad + b.row * a.clear.grad_stride + on * a.clear.grad_stride;
+    if (bytes >= 16) { // (a row's last 16 bytes end with the row)
+        __builtin_nontemporal_store((u32x4_e)0, GLOBAL_PTR(u32x4_e, p + (v * 16 + 16 <= bytes ? v * 16 : bytes - 16)));
     } else {
-        for (uint32_t o = 0; o < a.clear.row_bytes; o += 2) *GLOBAL_PTR(uint16_t, p + o) = 0;
+        for (uint32_t o = 0; o < bytes; o += 2) *GLOBAL_PTR(uint16_t, p + o) = 0;
     }
 }
 
@@ -1063,13 +1090,12 @@ template <int ED, int EG, bool TINY> DEV void embed_join_body(const NboEmbedGrad
             for (uint32_t i = lo; i < hi; i += U) {
                 A x[U][V];
 #pragma unroll
-                for (int u = 0; u < U; u++)
-                    if (i + u < hi) load_slot<A, V>(slot_at<A, V>(a, k + 1 + i + u, SLOT_HEAD, v), x[u]);
+                for (int u = 0; u < U; u++) // (behind the run: its last one again)
+                    load_slot<A, V>(slot_at<A, V>(a, k + 1 + (i + u < hi ? i + u : hi - 1), SLOT_HEAD, v), x[u]);
 #pragma unroll
-                for (int u = 0; u < U; u++)
-                    if (i + u < hi)
+                for (int u = 0; u < U; u++) // (a select, no branch: into one the compiler would move the loads)
 #pragma unroll
-                        for (int j = 0; j < V; j++) acc[j] += x[u][j];
+                    for (int j = 0; j < V; j++) acc[j] += i + u < hi ? x[u][j] : (A)0;
             }
         }
         __syncthreads(); // (the boundary before has been read)

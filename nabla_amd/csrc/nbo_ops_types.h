@@ -71,10 +71,9 @@ struct NboRngAdvanceArgs {
 #define NBO_RADIX_TILE 4096u
 #define NBO_RADIX_BLOCK 512u
 #define NBO_RADIX_BITS 10u
-// Split and merge: ids per tile, and the widest range of keys, as a power of two (LDS of the merge: 4 bytes
-// for each wave and key).
+// Split and merge: ids per tile, and the most keys of a range (LDS of the merge: 4 bytes for each wave and key).
 #define NBO_SPLIT_TILE 1024u
-#define NBO_SPLIT_SHIFT 9u
+#define NBO_SPLIT_KEYS 512u
 // Up to this many ids the gradient is one launch that needs no order.
 #define NBO_EMBED_DIRECT_MAX 512u
 
@@ -87,11 +86,11 @@ struct NboClearArgs {
 
 // Largest table for which the ordering launches note the rows that have ids (one byte each); the radix passes
 // do not, and a launch of its own looks the rows up.
-#define NBO_NAMED_ROWS (1u << 21)
+#define NBO_NAMED_ROWS (NBO_RANGE_KEYS << 11)
 
 struct NboOrderArgs {
     NboClearArgs clear;    // nbo_order_clear
-    uint8_t *named;        // [rows] or null: whether a row has ids
+    uint8_t *named;        // [ranges][range] or null: whether a row has ids
     const void *ids;       // the caller's (first pass), or null: keys_in / pos_in
     const uint32_t *keys_in, *pos_in;
     uint32_t *keys_out, *pos_out;
@@ -101,8 +100,9 @@ struct NboOrderArgs {
     uint32_t rows;
     uint32_t ids64;
     uint32_t tiles;
-    uint32_t shift, digits; // this pass's digit: (key >> shift) & (digits - 1); of the split: key >> shift
-    uint32_t range;         // keys per workgroup (order by ranges)
+    uint32_t shift, digits; // radix passes: this pass's digit is (key >> shift) & (digits - 1); otherwise: key v is
+                            // number v >> shift of range v % 2^shift, and `digits` ranges have keys
+    uint32_t range;         // keys per range
     uint32_t pad;
 };
 
@@ -115,7 +115,8 @@ struct NboEmbedGradArgs {
     uint64_t dy_stride, grad_stride; // bytes
     NboClearArgs clear;
     NboUnits clear_units;         // 16 bytes each
-    const uint8_t *named;
+    const uint8_t *named;         // [ranges][named_range]: whether a row has ids
+    uint32_t named_shift, named_range;
     double scale;
     uint32_t n, rows, cols;
     uint32_t units;               // per row
