@@ -72,7 +72,7 @@ static const char *const kKernelNames[K_COUNT] = {
     "nbo_embed_direct_f32",        "nbo_embed_direct_bf16",      "nbo_embed_direct_f64",
     "nbo_embed_direct_f16",        "nbo_embed_direct_bf16_f32",  "nbo_embed_direct_f16_f32",
     "nbo_dropout_f32",             "nbo_dropout_bf16",           "nbo_dropout_f64",
-    "nbo_dropout_f16",             "nbo_rng_advance",            "nbo_order_clear",
+    "nbo_dropout_f16",             "nbo_rng_advance",            "nbo_embed_clear",
 };
 static_assert(K_UPDATE_SELF_BASE + 18 == K_UPDATE_ROWS_BASE, "six families of three self-preparing update kernels");
 static_assert(K_UPDATE_ROWS_BASE + 8 == K_ACCSCALE_BASE && K_ACCSCALE_F16 + 3 == K_OPS_BASE,

@@ -83,7 +83,7 @@ enum KernelId {
     K_EMBED_DIRECT_BASE = 103, // + pair
     K_DROPOUT_BASE = 109,      // + element type (f32, bf16, f64, f16)
     K_RNG_ADVANCE = 113,
-    K_ORDER_CLEAR = 114,
+    K_EMBED_CLEAR = 114,
     K_COUNT = 115 // ids from here on are measurement kernels, handed out by Runtime::bench_kernel
 };
 

@@ -161,6 +161,11 @@ constexpr uint64_t PIECE_MAX = 64, PIECE_MIN = 8;
 // several (1023 boundaries and 8 slabs each: 13.4 us, one to a workgroup 15.8).
 constexpr uint64_t JOIN_WGS = 4096;
 
+// Above either the direct form's matrix is cleared ahead of it, by a launch that does nothing else and fills faster
+// (77 MB 14.6 us in one launch, 16.0 in two; 154 MB 28.5 and 26.7; 1051 MB 182 and 161; 131072 rows of 96 bytes 14.2
+// and 9.3, 50257 of 512 bytes 9.1 and 9.4).
+constexpr uint64_t CLEAR_FIRST_BYTES = 128ull << 20, CLEAR_FIRST_ROWS = 1ull << 16;
+
 // lanes that work on one piece
 uint64_t piece_lanes(uint64_t units)
 {
@@ -205,13 +210,21 @@ uint32_t range_shift(uint64_t rows, uint64_t keys)
     return shift;
 }
 
-// The tokens ordered by rows into (keys, pos) of the workspace; returns which of the two buffers.  With rows to
-// clear, g.named says which rows have ids, or is null and they have been cleared.
+void launch_clear(NboClearArgs c, uint64_t rows)
+{
+    if (c.grad_stride == c.row_bytes && rows * c.row_bytes >= 16) { // (with no rows to leave alone, whatever their width)
+        c.flat_bytes = rows * c.row_bytes;
+        c.u.total = ceil_div(c.flat_bytes, 16);
+    }
+    Runtime::get().launch_folded(K_EMBED_CLEAR, grid_of(c.u.total, NBO_OPS_BLOCK), NBO_OPS_BLOCK, c);
+}
+
+// The tokens ordered by rows into (keys, pos) of the workspace; returns which of the two buffers.  With a matrix
+// to clear, g.named says afterwards which rows have ids, or is null and it has been cleared.
 int launch_order(const nbo_ids &ids, uint64_t rows, nbo_embedding_ws *ws, NboEmbedGradArgs &g)
 {
     Runtime &rt = Runtime::get();
     NboOrderArgs a = {};
-    a.clear = g.clear;
     a.ids = ids.data;
     a.ids64 = ids.type == NBO_ID_I64;
     a.n = (uint32_t)ids.n;
@@ -224,8 +237,8 @@ int launch_order(const nbo_ids &ids, uint64_t rows, nbo_embedding_ws *ws, NboEmb
         a.range = (uint32_t)((rows - 1) >> shift) + 1;
         a.named = g.clear.grad ? ws->named : nullptr;
         g.named = a.named;
-        g.named_shift = a.shift;
-        g.named_range = a.range;
+        g.clear.named_shift = a.shift;
+        g.clear.named_range = a.range;
     };
     if (ids.n <= NBO_RANGE_IDS && rows <= NBO_NAMED_ROWS) {
         deal_out(range_shift(rows, NBO_RANGE_KEYS));
@@ -247,6 +260,7 @@ int launch_order(const nbo_ids &ids, uint64_t rows, nbo_embedding_ws *ws, NboEmb
         rt.launch(K_ORDER_MERGE, a.digits, NBO_RANGE_BLOCK, a);
         return 0;
     }
+    if (g.clear.grad) launch_clear(g.clear, rows);
     const int bits = bits_of(rows); // (the key of ids outside the table is `rows` itself)
     const int passes = (bits + NBO_RADIX_BITS - 1) / NBO_RADIX_BITS;
     const int per = (bits + passes - 1) / passes;
@@ -263,10 +277,6 @@ int launch_order(const nbo_ids &ids, uint64_t rows, nbo_embedding_ws *ws, NboEmb
         rt.launch(K_ORDER_HIST, a.tiles, NBO_RADIX_BLOCK, a);
         rt.launch(K_ORDER_SCAN, a.digits, 64, a);
         rt.launch(K_ORDER_SCATTER, a.tiles, NBO_RADIX_BLOCK, a);
-    }
-    if (g.clear.grad) {
-        a.keys_in = ws->keys[to];
-        rt.launch_folded(K_ORDER_CLEAR, grid_of(rows, NBO_CLEAR_ROWS * NBO_OPS_BLOCK / 64), NBO_OPS_BLOCK, a);
     }
     return to;
 }
@@ -419,13 +429,21 @@ int nbo_embedding_grad(const nbo_matrix *grad_out, const nbo_ids *ids, double sc
         a.ids64 = ids->type == NBO_ID_I64;
         const uint64_t waves_per_wg = NBO_OPS_BLOCK / 64;
         if (!accumulate) {
-            a.clear = NboClearArgs{grad->data, a.grad_stride, grad->cols * size_of(grad->dtype)};
-            a.clear_units = units_of(grad->rows, ceil_div(a.clear.row_bytes, 16));
+            a.clear.grad = grad->data;
+            a.clear.grad_stride = a.grad_stride;
+            a.clear.row_bytes = grad->cols * size_of(grad->dtype);
+            a.clear.u = units_of(grad->rows, ceil_div(a.clear.row_bytes, 16));
+            if (a.grad_stride == a.clear.row_bytes && a.clear.row_bytes % 16 == 0) a.clear.flat_bytes = grad->rows * a.clear.row_bytes;
         }
         if (ids->n <= NBO_EMBED_DIRECT_MAX) {
             a.ids = ids->data;
             a.sum_wgs = grid_of(ids->n * a.slabs, 1);
-            const uint32_t clear_wgs = accumulate ? 0 : grid_of(grad->rows, NBO_CLEAR_ROWS * waves_per_wg);
+            if (a.clear.grad && (grad->rows * a.clear.row_bytes > CLEAR_FIRST_BYTES || grad->rows > CLEAR_FIRST_ROWS)) {
+                launch_clear(a.clear, grad->rows);
+                a.clear.grad = nullptr;
+                if (ids->n == 0) return;
+            }
+            const uint32_t clear_wgs = a.clear.grad ? grid_of(grad->rows, NBO_CLEAR_ROWS * waves_per_wg) : 0;
             rt.launch_folded(K_EMBED_DIRECT_BASE + pair, grid_of((uint64_t)a.sum_wgs + clear_wgs, 1), NBO_OPS_BLOCK, a);
             return;
         }
@@ -436,13 +454,12 @@ int nbo_embedding_grad(const nbo_matrix *grad_out, const nbo_ids *ids, double sc
         const uint64_t need = 2ull * a.pieces * a.units * unit * (grad->dtype == NBO_DT_F64 ? 8 : 4);
         require(need <= ws->partial_bytes, NBO_ERR_TOO_LARGE, "internal: the workspace's partial sums are too small");
         const int order = launch_order(*ids, grad->rows, ws, a);
-        if (!a.named) a.clear.grad = nullptr;
         a.keys = ws->keys[order];
         a.pos = ws->pos[order];
         a.partial = ws->partial;
         const uint64_t waves = a.lanes == 64 ? (uint64_t)a.pieces * a.slabs : ceil_div(a.pieces, 64 / a.lanes);
         a.sum_wgs = grid_of(waves, waves_per_wg);
-        const uint32_t clear_wgs = a.clear.grad ? grid_of(a.clear_units.total, NBO_OPS_BLOCK) : 0;
+        const uint32_t clear_wgs = a.named ? grid_of(a.clear.u.total, NBO_OPS_BLOCK) : 0;
         rt.launch_folded(K_EMBED_SUM_BASE + pair, grid_of((uint64_t)a.sum_wgs + clear_wgs, 1), NBO_OPS_BLOCK, a);
         // (more ids than the direct form takes are at least nine pieces)
         const uint64_t edges = a.pieces - 1;

@@ -5,7 +5,7 @@
 //   nbo_order_range    the tokens ordered by rows, in one launch (up to 8192 ids)
 //   nbo_order_split / _merge             ... in two (more ids)
 //   nbo_order_hist / _scan / _scatter    ... by radix passes (tables of more than half a million rows)
-//   nbo_order_clear    zeros in the rows no id names, behind the radix passes
+//   nbo_embed_clear    zeros everywhere, ahead of the sums: large tables of which few rows are named
 //   nbo_embed_sum_*    grad[v] (+)= scale * sum of the rows of dy that name v, in pieces of the order; zeros in the
 //                      rows no id names
 //   nbo_embed_join_*   ... of the rows whose tokens span pieces
@@ -783,54 +783,6 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
     fill_padding(a, total_of<WAVES>(wvalid), blockIdx.x, a.digits);
 }
 
-// First place in keys[lo .. hi) whose key is not below `key`
-DEV uint32_t lower_bound(const uint32_t *keys, uint32_t lo, uint32_t hi, uint32_t key)
-{
-    while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (GLOBAL_PTR(const uint32_t, keys)[mid] < key) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo;
-}
-// ... by a whole wave, 64 places at a time
-DEV uint32_t lower_bound_wave(const uint32_t *keys, uint32_t n, uint32_t key)
-{
-    const uint32_t lane = threadIdx.x & 63u;
-    uint32_t lo = 0, len = n; // the place is in [lo, lo + len]
-    while (len > 0) {
-        const uint32_t step = (len + 63) / 64;
-        const uint64_t i = (uint64_t)lo + (uint64_t)lane * step;
-        const bool below = lane * (uint64_t)step < len && GLOBAL_PTR(const uint32_t, keys)[i] < key;
-        const uint32_t c = (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(below)); // probes 0 .. c - 1 are below
-        if (c == 0) return lo;
-        const uint32_t from = (c - 1) * step + 1; // behind the last probe that is below
-        const uint32_t to = c * step < len ? c * step : len;
-        lo += from;
-        len = to > from ? to - from : 0;
-    }
-    return lo;
-}
-
-// After the radix passes: zeros in the rows no id names, a few rows to a wave.
-extern "C" __global__ __launch_bounds__(NBO_OPS_BLOCK) void nbo_order_clear(const NboOrderArgs a)
-{
-    enum { ROWS = NBO_CLEAR_ROWS };
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t from = ((uint64_t)folded_workgroup() * (NBO_OPS_BLOCK / 64) + threadIdx.x / 64) * ROWS;
-    if (from >= a.rows) return;
-    const uint32_t count = a.rows - from < ROWS ? (uint32_t)(a.rows - from) : ROWS;
-    const uint32_t lo = lower_bound_wave(a.keys_in, a.n, (uint32_t)from);
-    const uint32_t hi = lower_bound_wave(a.keys_in, a.n, (uint32_t)from + count);
-    bool here = false;
-    if (lo < hi && lane < count) {
-        const uint32_t at = lower_bound(a.keys_in, lo, hi, (uint32_t)from + lane);
-        here = at < hi && GLOBAL_PTR(const uint32_t, a.keys_in)[at] == (uint32_t)from + lane;
-    }
-    const uint64_t named = __builtin_amdgcn_ballot_w64(here);
-    clear_rows(a.clear, from, count, named);
-}
-
 // ---------------------------------------------------------------------------------
 // The sums.  The order is cut into pieces of a.piece tokens; `lanes` lanes, one unit of the row each,
 // walk a piece and add up the rows of dy.  A row of the table all of whose tokens lie in the piece is
@@ -1002,23 +954,30 @@ template <int ED, int EG> DEV void sum_wide(const NboEmbedGradArgs &a, uint32_t 
     }
 }
 
-// Zeros in the rows that no id names: one 16-byte store per thread and its wave is gone, through the
-// matrix from the front -- the shape in which this memory takes a fill fastest (6.6 TB/s over 1 GiB; waves that
-// walk ranges of their own 5.0-5.8).
-DEV void clear_unnamed(const NboEmbedGradArgs &a, uint32_t wg)
+// Zeros through the matrix from the front, one 16-byte store per thread and its wave is gone -- the shape in
+// which this memory takes a fill fastest (6.6 TB/s over 1 GiB; waves that walk ranges of their own 5.0-5.8).
+// `named`, if given, says which rows to leave alone.
+DEV void clear_units(const NboClearArgs &c, const uint8_t *named, uint32_t wg)
 {
     const uint64_t base = (uint64_t)wg * NBO_OPS_BLOCK;
-    if (base + threadIdx.x >= a.clear_units.total) return;
-    const UnitBase b = unit_base(a.clear_units, base);
-    uint32_t on, v;
-    unit_from(a.clear_units, b, threadIdx.x, &on, &v);
-    const uint32_t row = (uint32_t)b.row + on, bytes = (uint32_t)a.clear.row_bytes;
-    if (GLOBAL_PTR(const uint8_t, a.named)[(row & ((1u << a.named_shift) - 1)) * a.named_range + (row >> a.named_shift)]) return;
-    if (bytes % 16 == 0 && a.clear.grad_stride == bytes) { // units follow one another: few instructions per store
-        __builtin_nontemporal_store((u32x4_e)0, GLOBAL_PTR(u32x4_e, (char *)a.clear.grad + base * 16 + threadIdx.x * 16));
+    if (base + threadIdx.x >= c.u.total) return;
+    UnitBase b = {};
+    uint32_t on = 0, v = 0;
+    if (named || !c.flat_bytes) {
+        b = unit_base(c.u, base);
+        unit_from(c.u, b, threadIdx.x, &on, &v);
+    }
+    if (named) {
+        const uint32_t row = (uint32_t)b.row + on;
+        if (GLOBAL_PTR(const uint8_t, named)[(row & ((1u << c.named_shift) - 1)) * c.named_range + (row >> c.named_shift)]) return;
+    }
+    if (c.flat_bytes) { // (few instructions per store; the last 16 bytes end with the matrix)
+        const uint64_t o = (base + threadIdx.x) * 16;
+        __builtin_nontemporal_store((u32x4_e)0, GLOBAL_PTR(u32x4_e, (char *)c.grad + (o + 16 <= c.flat_bytes ? o : c.flat_bytes - 16)));
         return;
     }
-    char *p = (char *)a.clear.grad + b.row * a.clear.grad_stride + on * a.clear.grad_stride;
+    const uint32_t bytes = (uint32_t)c.row_bytes;
+    char *p = (char *)c.grad + b.row * c.grad_stride + on * c.grad_stride;
     if (bytes >= 16) { // (a row's last 16 bytes end with the row)
         __builtin_nontemporal_store((u32x4_e)0, GLOBAL_PTR(u32x4_e, p + (v * 16 + 16 <= bytes ? v * 16 : bytes - 16)));
     } else {
@@ -1026,11 +985,16 @@ DEV void clear_unnamed(const NboEmbedGradArgs &a, uint32_t wg)
     }
 }
 
+extern "C" __global__ __launch_bounds__(NBO_OPS_BLOCK) void nbo_embed_clear(const NboClearArgs c)
+{
+    clear_units(c, nullptr, folded_workgroup());
+}
+
 template <int ED, int EG, bool TINY> DEV void embed_sum_body(const NboEmbedGradArgs &a)
 {
     const uint32_t wg = folded_workgroup();
     if (wg >= a.sum_wgs) {
-        if (a.clear.grad) clear_unnamed(a, wg - a.sum_wgs);
+        if (a.named) clear_units(a.clear, a.named, wg - a.sum_wgs);
         return;
     }
     const uint32_t wave = wg * (NBO_OPS_BLOCK / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);

@@ -77,19 +77,23 @@ struct NboRngAdvanceArgs {
 // Up to this many ids the gradient is one launch that needs no order.
 #define NBO_EMBED_DIRECT_MAX 512u
 
-// Rows to clear: those of grad that no id names (grad null: none).
-#define NBO_CLEAR_ROWS 4u // per wave, where it has to find out which
+// Rows dealt out to ranges: row v is number v >> shift of range v % 2^shift.
+
+// The matrix to clear, in units of 16 bytes.
+#define NBO_CLEAR_ROWS 4u // per wave, in the direct form
 struct NboClearArgs {
-    void *grad;
+    void *grad; // null: none
     uint64_t grad_stride, row_bytes;
+    uint64_t flat_bytes; // of a matrix whose units follow one another, or 0
+    NboUnits u;
+    uint32_t named_shift, named_range; // how `named` is laid out: [ranges][named_range] bytes, whether a row has ids
 };
 
-// Largest table for which the ordering launches note the rows that have ids (one byte each); the radix passes
-// do not, and a launch of its own looks the rows up.
+// Largest table for which the ordering launches note the rows that have ids (one byte each).  Larger ones are
+// cleared as a whole, ahead of the sums.
 #define NBO_NAMED_ROWS (NBO_RANGE_KEYS << 11)
 
 struct NboOrderArgs {
-    NboClearArgs clear;    // nbo_order_clear
     uint8_t *named;        // [ranges][range] or null: whether a row has ids
     const void *ids;       // the caller's (first pass), or null: keys_in / pos_in
     const uint32_t *keys_in, *pos_in;
@@ -100,8 +104,8 @@ struct NboOrderArgs {
     uint32_t rows;
     uint32_t ids64;
     uint32_t tiles;
-    uint32_t shift, digits; // radix passes: this pass's digit is (key >> shift) & (digits - 1); otherwise: key v is
-                            // number v >> shift of range v % 2^shift, and `digits` ranges have keys
+    uint32_t shift, digits; // radix passes: this pass's digit is (key >> shift) & (digits - 1); otherwise 2^shift
+                            // ranges, of which `digits` have rows
     uint32_t range;         // keys per range
     uint32_t pad;
 };
@@ -114,9 +118,7 @@ struct NboEmbedGradArgs {
     void *partial;                // [pieces][2][units * VEC] sums of rows that span pieces
     uint64_t dy_stride, grad_stride; // bytes
     NboClearArgs clear;
-    NboUnits clear_units;         // 16 bytes each
-    const uint8_t *named;         // [ranges][named_range]: whether a row has ids
-    uint32_t named_shift, named_range;
+    const uint8_t *named;         // whether a row has ids (null: nothing to clear)
     double scale;
     uint32_t n, rows, cols;
     uint32_t units;               // per row

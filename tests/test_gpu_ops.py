@@ -244,6 +244,21 @@ def test_embedding_grad_of_views_writes_nothing_else(gpu, pair, n):
         assert torch.equal(big[:, :7], before[:, :7]) and torch.equal(big[:, 7 + cols:], before[:, 7 + cols:])
 
 
+@pytest.mark.parametrize("rows,cols,stride,dtype", [(65536, 7, 7, "f32"), (65537, 7, 7, "f32"), (70001, 1, 1, "f16"),
+                                                    (70001, 3, 5, "f16"), (70001, 1, 2, "f64"), (70000, 1000, 1031, "bf16"),
+                                                    (70003, 1031, 1031, "bf16"), (70000, 16, 16, "bf16"), (2000003, 2, 3, "f32"),
+                                                    (1966080, 1, 1, "f32"), (1966081, 9, 9, "f16")])
+@pytest.mark.parametrize("n", [0, 5, 512, 600])
+def test_embedding_grad_clears_large_matrices(gpu, rows, cols, stride, dtype, n):
+    """Fresh gradients of matrices that are cleared ahead of the sums, with gaps between the rows and without."""
+    big = torch.full((rows, stride), 3.0, device=DEV, dtype=T[dtype])
+    ids = rand_ids(n, rows, 2, 0.1)
+    if n:
+        ids[0], ids[-1] = rows - 1, 0
+    check_grad(randn(n, cols, dtype, 1), ids, big[:, :cols], ops.EmbeddingWorkspace(n, cols))
+    assert torch.equal(big[:, cols:], torch.full_like(big[:, cols:], 3.0))
+
+
 def test_embedding_grad_against_differences(gpu):
     """d(sum of c * embedding) / d(table) by central differences in f64: the operator is linear in the
     table, so they are exact up to rounding."""
