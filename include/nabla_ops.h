@@ -52,7 +52,7 @@ typedef struct nbo_ids {
 int nbo_embedding(const nbo_matrix *table, const nbo_ids *ids, const nbo_matrix *add, double scale,
                   const nbo_matrix *out);
 
-/* Scratch of nbo_embedding_grad for up to max_ids ids and max_cols columns: the ids in table order
+/* Scratch of nbo_embedding_grad for up to max_ids ids and max_cols columns: the ids ordered by rows
  * and partial sums of rows that many tokens name.  Nothing in it outlives a call, but two calls
  * that run at the same time (two captured graphs on two streams) need one each. */
 typedef struct nbo_embedding_ws nbo_embedding_ws;
@@ -62,9 +62,9 @@ int nbo_embedding_ws_destroy(nbo_embedding_ws *ws);
 /* The gradient of nbo_embedding with respect to the table:
  *   grad[v] = (accumulate ? grad[v] : 0) + scale * sum of grad_out[t] over the t with ids[t] == v
  * With accumulate == 0 every row is written, zeros where no id names it; otherwise the rows no id
- * names are not touched.  What rows of grad_out hold whose id is outside the table does not matter.  Sums are
- * f32 (f64 lists: f64), over the tokens in a fixed order -- the same bits on every run -- and
- * rounded once, to grad's type: grad_out's, or f32 over bf16 / f16.  (With respect to `add` the
+ * names are not touched.  What rows of grad_out hold whose id is outside the table does not matter.
+ * Sums are f32 (f64 tensors: f64), over the tokens in a fixed order -- the same bits on every run --
+ * and rounded once, to grad's type: grad_out's, or f32 over bf16 / f16.  (With respect to `add` the
  * gradient is grad_out itself.)  grad may not overlap grad_out or the ids.  Asynchronous. */
 int nbo_embedding_grad(const nbo_matrix *grad_out, const nbo_ids *ids, double scale, int accumulate,
                        const nbo_matrix *grad, nbo_embedding_ws *ws);
@@ -87,8 +87,8 @@ int nbo_rng_advance(nbo_rng *rng, uint64_t steps); /* step += steps (modulo 2^64
  * rate that is applied, so the mean is exact.  0 <= p <= 1 (NBO_ERR_ARG); p = 1 drops everything.
  * Element e = row * cols + col is dropped if its 16 bits of Philox4x32-10 are below thr: key = seed;
  * counter = (e / 8, site, step's low half, step's high half); the bits are half e % 2 (low first) of
- * word e % 8 / 2.  `site` tells the dropouts of one step apart (one number per place in the model).  A dropped element is zero whatever x
- * holds there (inf, NaN).  The gradient is the same call on the gradient, without residual, at the
+ * word e % 8 / 2.  `site` tells the dropouts of one step apart (one number per place in the model).  A
+ * dropped element is zero whatever x holds there (inf, NaN).  The gradient is the same call on the gradient, without residual, at the
  * same seed, step and site.  Computed in f32 (f64: f64), rounded once.  x, residual and out have one
  * shape and type; out may be x or residual itself, other overlaps are NBO_ERR_ARG.  At most 2^35
  * elements.  Asynchronous. */

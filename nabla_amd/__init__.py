@@ -1,6 +1,6 @@
 """nabla_amd -- MI355X (gfx950) fused optimizer-step engine for fumishiki/nabla.
 
-Only the optimizer-step path is here: ``nabla_amd.optim`` mirrors
+The optimizer-step path, and beside it three operators on the same tensors: ``nabla_amd.optim`` mirrors
 nabla-train's ``Sgd`` / ``Adam`` / ``AdamW`` / ``GradScaler`` /
 ``clip_grad_norm`` / ``zero_grad`` over the C ABI of ``include/nabla_optim.h``
 (``libnabla_optim.so``: hand-written HIP kernels, embedded gfx950 code object);
@@ -8,7 +8,8 @@ nabla-train's ``Sgd`` / ``Adam`` / ``AdamW`` / ``GradScaler`` /
 ``nabla_amd.trainer`` (the Trainer's loop body after backward) and
 ``nabla_amd.checkpoint`` (NBLA / meta.txt) are the callers and file formats
 either side of it; ``nabla_amd.backend`` is nabla-core's Backend primitives as
-multi-tensor launches.
+multi-tensor launches; ``nabla_amd.ops`` (C ABI: ``include/nabla_ops.h``) is the
+embedding lookup, its gradient, and dropout.
 """
 from . import _lib  # noqa: F401
 from .optim import (Adam, AdamW, GradScaler, GradScalerState, NablaPanic, OptimMeta,  # noqa: F401

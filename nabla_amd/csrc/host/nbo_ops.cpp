@@ -153,8 +153,9 @@ uint64_t unit_elems(int a, int b) { return 16 / std::min(size_of(a), size_of(b))
 
 // ---- the gradient's plan -------------------------------------------------------------------
 
-// Ids per piece: as many of 64, 32, 16 as leave SUM_WAVES waves to the chip, or 8 (a piece's waves walk
-// it one id after the other).
+// Ids per piece: as many of 64, 32, 16 as leave SUM_WAVES waves to the chip, or 8: a piece's waves walk it one
+// id after the other, and every piece leaves sums to the join (65536 rows of 512 bf16: 52.7 us with 2048 waves, 51.5
+// with 4096, 56.7 with 8192; 16384 of 2048: 46.6, 44.4, 47.2).
 constexpr uint64_t SUM_WAVES = 4096;
 constexpr uint64_t PIECE_MAX = 64, PIECE_MIN = 8;
 // Most workgroups of the join, 16 for each compute unit; with more boundaries than that a workgroup looks at

@@ -217,7 +217,10 @@ template <int U> DEV void load_keys(const void *ids, uint32_t ids64, const uint6
 }
 
 // ---------------------------------------------------------------------------------
-// The lookup: U units per thread, all ids read, then all rows, then all stores.
+// The lookup: U units per thread, all ids read, then all rows, then all stores.  Two loads that wait for one
+// another, the id and its row, so that what is in flight decides: 65536 rows of 8 KiB with one unit a thread 181 us,
+// two 149, four 131 (5.3 TB/s of rows and result; a copy in the best shape 6.65), eight 154.  Rows are kept in the
+// caches, for the ids that come again (past them: 176 us), the result is not.
 template <int ET, int EO, int U, bool TINY> DEV void embed_body(const NboEmbedArgs &a)
 {
     enum { V = Pair<ET, EO>::V, ST = sizeof(typename El<ET>::Bits), SO = sizeof(typename El<EO>::Bits) };
@@ -308,12 +311,15 @@ DEV uint32_t wave_scan(uint32_t x)
 // rows are dealt out to 2^shift ranges, row v to range v % 2^shift: ids that are close to one another (a
 // vocabulary sorted by frequency, positions) are spread over all ranges.  Ranges come in order, within a range the
 // rows, within a row its tokens; padding takes no part, and the places behind the last token hold its key.
-// (With ranges of adjacent rows the merge of 65536 ids, log-uniform over 131072 rows, took 57 us instead of NEW1.)
+// (With ranges of adjacent rows the merge of 65536 ids, log-uniform over 131072 rows in order of frequency, took
+// 57 us instead of 13.)  Where most ids are one row, one workgroup does most of the work, at the 25 GB/s that one
+// compute unit reads: 65536 ids of one row 45 us.
 //
 // In one launch: every workgroup owns a range, reads all ids and puts those of its range to their places.
 // Nothing passes between workgroups: how many ids come before the range is counted on the way.  Within the
 // range an id's place is its key's start, the ids of that key which earlier waves hold (each wave has a run of
-// the ids), and those its own wave has seen.
+// the ids), and those its own wave has seen.  The ids stay in registers from the first look at them to the
+// last.  8192 ids: 7.3 us, bound by latency and by the instructions that every workgroup spends on every id.
 
 // For a block of 64 ids of which the lanes in `left` (not empty) count: adds to mine[r] how many lanes hold
 // each r.  The lanes that hold what the first one holds are counted as one: an addition to one LDS word takes
@@ -493,8 +499,9 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_range(co
 }
 
 // ---------------------------------------------------------------------------------
-// Table order by stable radix passes of up to ten bits, least significant first.  Per pass: how often
-// each digit occurs in each tile; the running sums over the tiles, per digit; every id to its place.
+// Table order by stable radix passes of up to ten bits, least significant first, for tables with more rows than
+// the ranges hold.  Per pass: how often each digit occurs in each tile; the running sums over the tiles, per
+// digit; every id to its place.  65536 ids: 43 us in two passes, each three launches that wait for each other.
 template <int N> DEV void order_keys(const NboOrderArgs &a, const uint64_t (&t)[N], uint32_t (&key)[N])
 {
     if (!a.keys_in) {
@@ -634,7 +641,9 @@ extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_scatter(
 // ---------------------------------------------------------------------------------
 // The same order in two launches: every tile puts its ids in the order of the ranges, in place, and notes
 // where each range starts; then one workgroup per range collects it from all tiles and orders it as
-// nbo_order_range does.  What lies before the range is the sum of the tiles' starts.
+// nbo_order_range does.  What lies before the range is the sum of the tiles' starts.  Every id is moved twice
+// however many there are: 16384 ids 4.7 + 5.3 us, 65536 4.8 + 9.8, bound by latency (five loads and stores one
+// after the other).
 extern "C" __global__ __launch_bounds__(NBO_RADIX_BLOCK) void nbo_order_split(const NboOrderArgs a)
 {
     enum { WAVES = NBO_RADIX_BLOCK / 64, ROWS = NBO_SPLIT_TILE / NBO_RADIX_BLOCK };
@@ -788,7 +797,8 @@ extern "C" __global__ __launch_bounds__(NBO_RANGE_BLOCK) void nbo_order_merge(co
 // walk a piece and add up the rows of dy.  A row of the table all of whose tokens lie in the piece is
 // finished there; the sums of one that began in an earlier piece or goes on into the next are left in
 // the piece's two slots, for the join.  So a row that half the batch names is added up by many
-// waves, and in the same order of additions on every run.
+// waves, and in the same order of additions on every run.  Bound by memory: 65536 bf16 rows of 8 KiB into 128256,
+// with the zeros in the other rows, 276 us, 5.6 TB/s.
 template <int EG> DEV char *grad_at(const NboEmbedGradArgs &a, uint32_t key, const Span &s)
 {
     return (char *)a.grad + key * a.grad_stride + (uint64_t)s.c0 * sizeof(typename El<EG>::Bits);
@@ -901,8 +911,8 @@ template <int ED, int EG, bool TINY> DEV void sum_narrow(const NboEmbedGradArgs 
 
 // One piece (of at most 64 tokens) and slab of 64 units by a wave.  Lane i holds token i's key and
 // place, so that which token is the last of its row is one mask, and the rows' addresses are scalars.
-// (Asking for what the finished rows hold together with the tokens' rows, instead of at the row's end, measured
-// slower: 34-36 us against 31.4 for 16384 bf16 rows of 4 KiB into f32.)
+// Eight tokens' rows are asked for at a time.  (Asking for what the finished rows hold together with them, instead of
+// at the row's end, measured slower: 34-36 us against 31.4 for 16384 bf16 rows of 4 KiB into f32.)
 template <int ED, int EG> DEV void sum_wide(const NboEmbedGradArgs &a, uint32_t wave)
 {
     enum { V = Pair<ED, EG>::V, SD = sizeof(typename El<ED>::Bits), U = 8 };
@@ -1006,8 +1016,9 @@ template <int ED, int EG, bool TINY> DEV void embed_sum_body(const NboEmbedGradA
 // k is finished by that boundary's workgroups, one per slab of the row; a workgroup looks at a.edges boundaries.
 // The row's sums are piece k's tail and the heads of the pieces behind, as many as begin with its key; the
 // workgroup's waves -- groups of a.lanes lanes, where a row has few units -- take a run of them each.
-// (65536 rows of 4096 bf16: 13-16 us, with a workgroup per boundary 16-19; of 48 bf16, whose most frequent row has
-// 760 sums: 16, with a wave for each run of them 23.  It waits for memory: boundary, row, sums, one after the other.)
+// It waits for memory, one load after the other: 8192 tokens 5.6 us, 65536 13.  A row that has most of the tokens
+// is one workgroup's per slab: 1024 sums of 2 KiB take 90 us, at the 23 GB/s that one compute unit reads -- more
+// waves did not help (92 us with eight, 94 with sixteen), and cost every other row.
 template <int ED, int EG, bool TINY> DEV void embed_join_body(const NboEmbedGradArgs &a)
 {
     enum { V = Pair<ED, EG>::V, U = 8 };
@@ -1077,7 +1088,9 @@ template <int ED, int EG, bool TINY> DEV void embed_join_body(const NboEmbedGrad
 
 // A few ids: one workgroup per token and slab of its row.  It reads all ids; unless an earlier token names
 // the same row it adds up the rows of all tokens that do, each wave those in its run of the ids.  The
-// workgroups behind clear the rows no token names.
+// workgroups behind clear the rows no token names.  One launch and three loads one after the other: 4.0 us for 96
+// bf16 rows of 4 KiB.  Accumulating f32 rows of 3 KiB, 512 tokens take 6.6 us a call, 513 in three launches 14.1; all
+// of one row, 9.9 and 12.4.
 template <int ED, int EG, bool TINY> DEV void embed_direct_body(const NboEmbedGradArgs &a)
 {
     enum { V = Pair<ED, EG>::V, SD = sizeof(typename El<ED>::Bits), WAVES = NBO_OPS_BLOCK / 64, U = 8 };
@@ -1194,7 +1207,8 @@ NBO_EMBED_GRAD_KERNELS(f16_f32, NBO_F16, NBO_F32)
 
 // ---------------------------------------------------------------------------------
 // Philox4x32-10 (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3",
-// SC 2011): ten rounds of two 32 x 32 -> 64 bit products.
+// SC 2011): ten rounds of two 32 x 32 -> 64 bit products.  A block of eight elements costs some 100 instructions,
+// which 16 bytes of bf16 hide: 32768 rows of 8 KiB 86.7 us, 6.2 TB/s of x and result.
 DEV void philox(uint32_t block, uint32_t site, const NboRngDev &r, uint32_t (&w)[4])
 {
     uint32_t c0 = block, c1 = site, c2 = (uint32_t)r.step, c3 = (uint32_t)(r.step >> 32);

@@ -5,7 +5,7 @@
 
 #include <stdint.h>
 
-// Units per thread of the lookup (65536 rows of 8 KiB: one 181 us, two 149, four 138, eight 154).
+// Units per thread of the lookup.
 #define NBO_EMBED_UNITS 4
 #define NBO_OPS_BLOCK 256u // threads of every operator kernel but the ordering ones
 
@@ -60,10 +60,11 @@ struct NboRngAdvanceArgs {
 };
 
 // ---- the gradient of the embedding ------------------------------------------------------
-// Keys: the ids, with every id outside the table replaced by `rows`, so that padding sorts last.
+// Keys: the ids, with every id outside the table replaced by `rows`; padding comes last.
 
-// Order by ranges: one launch, every workgroup reads all ids; threads, and the most ids (they stay in
-// registers) and keys per workgroup (LDS: 4 bytes for each wave and key).
+// Order in one launch, every workgroup reads all ids; threads, and the most ids (they stay in registers) and keys
+// per workgroup (LDS: 4 bytes for each wave and key).  The whole gradient of 8192 ids, 512 bf16 columns: 20.1 us, by
+// split and merge 22.2; of 4096 ids 18.1 and 21.2.
 #define NBO_RANGE_BLOCK 1024u
 #define NBO_RANGE_IDS 8192u
 #define NBO_RANGE_KEYS 960u
@@ -74,11 +75,11 @@ struct NboRngAdvanceArgs {
 // Split and merge: ids per tile, and the most keys of a range (LDS of the merge: 4 bytes for each wave and key).
 #define NBO_SPLIT_TILE 1024u
 #define NBO_SPLIT_KEYS 512u
-// Up to this many ids the gradient is one launch that needs no order.
+// Up to this many ids the gradient is one launch that needs no order (every workgroup holds all ids in registers;
+// 512 f32 rows of 3 KiB 6.6 us, 513 by way of an order 14.1).
 #define NBO_EMBED_DIRECT_MAX 512u
 
-// Rows dealt out to ranges: row v is number v >> shift of range v % 2^shift.
-
+// Rows are dealt out to ranges: row v is number v >> shift of range v % 2^shift.
 // The matrix to clear, in units of 16 bytes.
 #define NBO_CLEAR_ROWS 4u // per wave, in the direct form
 struct NboClearArgs {
@@ -114,7 +115,7 @@ struct NboEmbedGradArgs {
     const void *dy;
     void *grad;
     const void *ids;              // the direct form only
-    const uint32_t *keys, *pos;   // in table order
+    const uint32_t *keys, *pos;   // ordered by rows
     void *partial;                // [pieces][2][units * VEC] sums of rows that span pieces
     uint64_t dy_stride, grad_stride; // bytes
     NboClearArgs clear;

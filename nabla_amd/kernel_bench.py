@@ -356,7 +356,7 @@ def ops_main(args) -> None:
         _lib.check(L.nbo_profile_enable(0))
         print(f"| {name} | {shape} | {us:.1f} | {nbytes / 1e6:.2f} | {nbytes / us / 1e3:.0f} | {', '.join(parts)} |", flush=True)
 
-    order = ["nbo_order_range", "nbo_order_split", "nbo_order_merge"]
+    order = ["nbo_embed_clear", "nbo_order_range", "nbo_order_split", "nbo_order_merge"]
     for rows, cols, n, dtype, tag, gdtype, gtag in ((128256, 4096, 1, bf16, "bf16", bf16, "bf16"),
                                                     (50257, 768, 8192, f32, "f32", f32, "f32"),
                                                     (32000, 2048, 16384, bf16, "bf16", f32, "bf16_f32"),

@@ -3,6 +3,8 @@
 Tolerances are arithmetic, not measurements: u = 2^-24 is the rounding of an f32 operation (2^-53 of an
 f64 one), h = eps / 2 the rounding to the stored type, 2^-25 half of f16's smallest step.
 """
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -460,6 +462,8 @@ def test_dropout_of_more_units_than_32_bits(gpu):
     """2^32 units and a few: f64 elements two to a unit, 64 GiB in one run, in place."""
     rows, cols = (1 << 23) + 1, 1024
     n = rows * cols
+    gc.collect()
+    torch.cuda.empty_cache()
     if torch.cuda.mem_get_info(DEV)[0] < n * 8 + (1 << 30):
         pytest.skip("needs 65 GiB of free device memory")
     x = torch.ones(rows, cols, device=DEV, dtype=torch.float64)
