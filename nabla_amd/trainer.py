@@ -118,7 +118,9 @@ class TrainerTail:
             return self._consume(grads)
         finally:  # the micro-batch is over, stepped, skipped or in error
             self.rng.advance()
-            self.state.rng_state = (self.state.rng_state + 1) % (1 << 64)
+            at = self.state.rng_state
+            # (a state put in place without a step: from the device, this once)
+            self.state.rng_state = self.rng.state().step if at is None else (at + 1) % (1 << 64)
 
     def _consume(self, grads) -> bool:
         grads = grads if isinstance(grads, nb.TensorList) else list(grads)

@@ -429,6 +429,18 @@ def test_generator_state(gpu):
 
 # ---- beyond 32 bits ------------------------------------------------------------------------
 
+@pytest.mark.parametrize("n", [40, 3000, 20000])
+def test_ids_beyond_32_bits_are_padding(gpu, n):
+    """Ids whose low halves are rows of the table."""
+    rows, cols = 50, 40
+    ids = rand_ids(n, rows, 1)
+    far = torch.tensor([1 << 32, -(1 << 32), 1 << 62, -(1 << 63)], device=DEV)[torch.arange(n, device=DEV) % 4]
+    ids = torch.where(torch.arange(n, device=DEV) % 3 == 0, ids + far, ids)
+    table = randn(rows, cols, "f32", 2)
+    check_embedding(table, ids, torch.empty(n, cols, device=DEV), 1.0, None)
+    check_grad(randn(n, cols, "f32", 3), ids, table, ops.EmbeddingWorkspace(n, cols))
+
+
 def test_offsets_beyond_32_bits(gpu):
     """Tables, batches and matrices of more than 2^32 elements: their last rows."""
     rows, cols = (1 << 22) + 3, 1032  # 4.3e9 elements, 8.7 GB
