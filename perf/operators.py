@@ -148,9 +148,9 @@ def _own(s):
         ops.embedding_grad(s["grad_out"], s["ids"], s["grad"], s["workspace"], scale=case["scale"],
                            accumulate=case["accumulate"])
         return s["grad"]
-    if case["backward"]:
+    if case["backward"] and s["residual"] is None:
         ops.dropout_grad(s["x"], case["p"], s["rng"], s["site"], s["out"])
-    else:
+    else:  # (a gradient that is added to another branch's is the same call, with that as residual)
         ops.dropout(s["x"], case["p"], s["rng"], s["site"], s["out"], residual=s["residual"])
     return s["out"]
 
