@@ -169,5 +169,6 @@ def dropout(x, p: float, rng: DropoutRng, site: int, out, residual=None) -> None
 
 def dropout_grad(grad_out, p: float, rng: DropoutRng, site: int, out) -> None:
     """The gradient of `dropout` with respect to x, at the same step and site of `rng`: grad_out
-    through the same mask and factor.  (With respect to `residual` it is grad_out itself.)"""
+    through the same mask and factor.  (With respect to `residual` it is grad_out itself; to add what
+    reaches x by other ways, call `dropout` with that as `residual`.)"""
     dropout(grad_out, p, rng, site, out)
