@@ -212,6 +212,15 @@ def test_embedding_grad_table_sizes(gpu, rows, n):
     check_grad(randn(n, 3, "f16", 1), ids.int(), randn(rows, 3, "f16", 2), ws, 1.0, True, "accumulated")
 
 
+@pytest.mark.parametrize("rows,step,n", [(60000, 256, 700), (60000, 256, 8192), (131072, 256, 8193), (131072, 256, 70000),
+                                         (400000, 1024, 30000), (131072, 128, 70000), (1900000, 2048, 5000)])
+def test_embedding_grad_of_ids_that_fall_into_one_range(gpu, rows, step, n):
+    """Ids a power of two apart: one workgroup of the order has all of them, the others none."""
+    ids = rand_ids(n, (rows - 1) // step + 1, 5, hot=True) * step + step // 2
+    ids = torch.where(torch.arange(n, device=DEV) % 13 == 0, -1, ids)
+    check_grad(randn(n, 20, "bf16", 1), ids, randn(rows, 20, "bf16", 2), ops.EmbeddingWorkspace(n, 20))
+
+
 def test_embedding_grad_does_not_read_padded_rows(gpu):
     for n in (200, 2000, 20000):
         ws = ops.EmbeddingWorkspace(n, 24)
