@@ -38,12 +38,43 @@ class CheckpointError(Exception):
 
 @dataclass
 class TrainState:
-    """trainer.rs TrainState: epoch, step, grad_accum, rng_state."""
+    """trainer.rs TrainState: epoch, step, grad_accum, rng_state.
+
+    A state that follows a generator (`TrainerTail.with_rng`) has its step as `rng_state`: read from the device
+    when it is asked for, because replays of a captured graph advance the generator without the host, and
+    loaded into it when it is set.  Copies hold the number it had."""
 
     epoch: int = 0
     step: int = 0
     grad_accum: int = 1
     rng_state: Optional[int] = None
+
+    def follow(self, rng) -> None:
+        """`rng_state` is the step of `rng` from here on; with None, the number it has now."""
+        at = self.rng_state
+        self._rng = rng
+        if rng is None or at is not None:
+            self.rng_state = at
+
+    def __getstate__(self):  # copies and pickles: plain values
+        return {"epoch": self.epoch, "step": self.step, "grad_accum": self.grad_accum, "rng_state": self.rng_state}
+
+    def _rng_state(self) -> Optional[int]:
+        return self.__dict__["rng_state"] if self._rng is None else self._rng.state().step
+
+    def _set_rng_state(self, step: Optional[int]) -> None:
+        if self._rng is None:
+            self.__dict__["rng_state"] = step
+        elif step is not None:  # (without one the generator goes on from where it is)
+            at = self._rng.state()
+            if at.step != step:
+                at.step = step
+                self._rng.load_state(at)
+
+
+# (behind the dataclass, to which they would be the fields' defaults)
+TrainState._rng = None
+TrainState.rng_state = property(TrainState._rng_state, TrainState._set_rng_state)
 
 
 def _to_host_f64(t) -> np.ndarray:
@@ -112,8 +143,9 @@ def write_meta(path: str, optimizer, scaler: Optional[GradScaler], schedule: Opt
                state: TrainState) -> None:
     """checkpoint.rs:107-150."""
     lines = ["version=1", f"epoch={state.epoch}", f"step={state.step}", f"grad_accum={state.grad_accum}"]
-    if state.rng_state is not None:
-        lines.append(f"rng.state={state.rng_state}")
+    rng_state = state.rng_state
+    if rng_state is not None:
+        lines.append(f"rng.state={rng_state}")
     lines += [f"{k}={v}" for k, v in optimizer.meta_pairs()]
     if schedule is not None:
         lines += [f"{k}={v}" for k, v in schedule_pairs(schedule)]

@@ -22,7 +22,9 @@ the two decisions stay separate entry points in the reference's order.
 
 A generator given with `with_rng` (nabla_amd.ops.DropoutRng) is advanced once per micro-batch,
 whatever became of it, so that the dropouts of the next one draw other masks; its step is
-`state.rng_state`, which checkpoints carry (checkpoint.rs:107-150, `rng.state`).
+`state.rng_state`, which checkpoints carry (checkpoint.rs:107-150, `rng.state`).  The device has the
+only copy: whatever else advances or loads the generator, a replayed graph among it, a checkpoint has
+the step that the next mask is drawn with.
 """
 from __future__ import annotations
 
@@ -54,7 +56,7 @@ class TrainerTail:
         self.grad_clip: Optional[float] = None
         self.nan_policy: Optional[GradNanPolicy] = None
         self.rng = None
-        self.state = TrainState(epoch=0, step=0, grad_accum=1, rng_state=None)
+        self._state = TrainState(epoch=0, step=0, grad_accum=1, rng_state=None)
         self._accum = None
         self._accum_count = 0
 
@@ -83,22 +85,22 @@ class TrainerTail:
         """`rng`: the ops.DropoutRng whose step one micro-batch's forward and backward pass share.
         Where a checkpoint has left a step in `state`, the generator goes on from there."""
         self.rng = rng
-        self._load_rng()
+        self._state.follow(rng)
         return self
 
-    def _load_rng(self) -> None:
-        if self.rng is None:
-            return
-        at = self.rng.state()
-        if self.state.rng_state is None:
-            self.state.rng_state = at.step
-        elif at.step != self.state.rng_state:
-            at.step = self.state.rng_state
-            self.rng.load_state(at)
+    @property
+    def state(self) -> TrainState:
+        return self._state
+
+    @state.setter
+    def state(self, state: TrainState) -> None:
+        if state is not self._state:
+            self._state.follow(None)
+            self._state = state
+        self._state.follow(self.rng)
 
     def set_state(self, state: TrainState) -> None:
         self.state = state
-        self._load_rng()
 
     def schedule_state(self) -> Optional[ScheduleState]:
         return self.schedule
@@ -118,9 +120,6 @@ class TrainerTail:
             return self._consume(grads)
         finally:  # the micro-batch is over, stepped, skipped or in error
             self.rng.advance()
-            at = self.state.rng_state
-            # (a state put in place without a step: from the device, this once)
-            self.state.rng_state = self.rng.state().step if at is None else (at + 1) % (1 << 64)
 
     def _consume(self, grads) -> bool:
         grads = grads if isinstance(grads, nb.TensorList) else list(grads)
