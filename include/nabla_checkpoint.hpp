@@ -3,7 +3,7 @@
 //
 // A checkpoint directory holds params.nbla and optim.nbla (tensor files, written and
 // read by the library straight from device memory: nbo_nbla_*_list, nbo_optim_*_state)
-// and meta.txt (key=value lines: version, epoch, step, grad_accum, rng.state, the
+// and meta.txt (key=value lines: version, epoch, step, grad_accum, rng.state, rng.seed, the
 // optimizer's meta pairs of optim/core.rs:263-324, the schedule's pairs of
 // core.rs:175-252, the scaler's state).  Floats are written the way Rust's Display prints
 // an f64: the shortest digits that round-trip, never in scientific notation.
@@ -33,10 +33,12 @@ struct CheckpointError : std::runtime_error {
     CheckpointError(std::string k, const std::string &m) : std::runtime_error(k + ": " + m), kind(std::move(k)) {}
 };
 
-// trainer.rs TrainState
+// trainer.rs TrainState; rng_seed goes with the step of a dropout generator (nabla_ops.hpp) and is a line of
+// meta.txt that the reference's reader passes over
 struct TrainState {
     uint64_t epoch = 0, step = 0, grad_accum = 1;
     std::optional<uint64_t> rng_state;
+    std::optional<uint64_t> rng_seed = std::nullopt;
 };
 
 // optim/core.rs:118-122
@@ -229,6 +231,7 @@ void write_meta(const std::string &path, Opt &optimizer, GradScaler *scaler, con
       << "step=" << state.step << "\n"
       << "grad_accum=" << state.grad_accum << "\n";
     if (state.rng_state) f << "rng.state=" << *state.rng_state << "\n";
+    if (state.rng_seed) f << "rng.seed=" << *state.rng_seed << "\n";
     for (const auto &kv : meta_pairs_of(optimizer)) f << kv.first << "=" << kv.second << "\n";
     if (schedule)
         for (const auto &kv : schedule_pairs(*schedule)) f << kv.first << "=" << kv.second << "\n";
@@ -293,9 +296,11 @@ template <typename Opt> MetaContents read_meta(const std::string &path, Opt &opt
                                      parse(detail::parse_f64, "scaler.backoff_factor"),
                                      parse(detail::parse_usize, "scaler.growth_interval"),
                                      parse(detail::parse_usize, "scaler.consecutive_ok")};
-    try {
-        out.state.rng_state = detail::parse_usize(m, "rng.state");
-    } catch (const StateError &) {
+    for (const auto &[key, value] : {std::pair{"rng.state", &out.state.rng_state}, std::pair{"rng.seed", &out.state.rng_seed}}) {
+        try {
+            *value = detail::parse_usize(m, key);
+        } catch (const StateError &) {
+        }
     }
     try {
         out.schedule = parse_schedule_state(m);

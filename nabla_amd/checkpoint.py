@@ -15,7 +15,7 @@ from __future__ import annotations
 
 import os
 import struct
-from dataclasses import dataclass
+from dataclasses import dataclass, fields
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -38,43 +38,52 @@ class CheckpointError(Exception):
 
 @dataclass
 class TrainState:
-    """trainer.rs TrainState: epoch, step, grad_accum, rng_state.
+    """trainer.rs TrainState: epoch, step, grad_accum, rng_state; and rng_seed, which the reference's has not.
 
-    A state that follows a generator (`TrainerTail.with_rng`) has its step as `rng_state`: read from the device
-    when it is asked for, because replays of a captured graph advance the generator without the host, and
-    loaded into it when it is set.  Copies hold the number it had."""
+    A state that follows a generator (`TrainerTail.with_rng`) has its step as `rng_state` and its seed as
+    `rng_seed`: read from the device when they are asked for, because replays of a captured graph advance the
+    generator without the host, and loaded into it when they are set.  Copies hold the numbers it had."""
 
     epoch: int = 0
     step: int = 0
     grad_accum: int = 1
     rng_state: Optional[int] = None
+    rng_seed: Optional[int] = None
 
     def follow(self, rng) -> None:
-        """`rng_state` is the step of `rng` from here on; with None, the number it has now."""
-        at = self.rng_state
+        """`rng_state` and `rng_seed` are those of `rng` from here on; with None, the numbers they are now.
+        What a checkpoint has left in them is loaded into `rng`; one that takes another's place goes on from
+        its step, with a seed of its own."""
+        step, seed = self.rng_state, self.rng_seed
+        if rng is not None and self._rng is not None:
+            seed = None
         self._rng = rng
-        if rng is None or at is not None:
-            self.rng_state = at
+        self.rng_state, self.rng_seed = step, seed
 
     def __getstate__(self):  # copies and pickles: plain values
-        return {"epoch": self.epoch, "step": self.step, "grad_accum": self.grad_accum, "rng_state": self.rng_state}
+        return {f.name: getattr(self, f.name) for f in fields(self)}
 
-    def _rng_state(self) -> Optional[int]:
-        return self.__dict__["rng_state"] if self._rng is None else self._rng.state().step
 
-    def _set_rng_state(self, step: Optional[int]) -> None:
+def _followed(name: str, part: str) -> property:
+    def get(self) -> Optional[int]:
+        return self.__dict__.get(name) if self._rng is None else getattr(self._rng.state(), part)
+
+    def put(self, value: Optional[int]) -> None:
         if self._rng is None:
-            self.__dict__["rng_state"] = step
-        elif step is not None:  # (without one the generator goes on from where it is)
+            self.__dict__[name] = value
+        elif value is not None:  # (without one the generator goes on from what it has)
             at = self._rng.state()
-            if at.step != step:
-                at.step = step
+            if getattr(at, part) != value:
+                setattr(at, part, value)
                 self._rng.load_state(at)
+
+    return property(get, put)
 
 
 # (behind the dataclass, to which they would be the fields' defaults)
 TrainState._rng = None
-TrainState.rng_state = property(TrainState._rng_state, TrainState._set_rng_state)
+TrainState.rng_state = _followed("rng_state", "step")
+TrainState.rng_seed = _followed("rng_seed", "seed")
 
 
 def _to_host_f64(t) -> np.ndarray:
@@ -141,11 +150,10 @@ def load_tensors(path: str) -> List[Tuple[str, np.ndarray]]:
 
 def write_meta(path: str, optimizer, scaler: Optional[GradScaler], schedule: Optional[ScheduleState],
                state: TrainState) -> None:
-    """checkpoint.rs:107-150."""
+    """checkpoint.rs:107-150; `rng.seed`, where the state has one, is a line that the reference's reader passes
+    over (it looks its keys up)."""
     lines = ["version=1", f"epoch={state.epoch}", f"step={state.step}", f"grad_accum={state.grad_accum}"]
-    rng_state = state.rng_state
-    if rng_state is not None:
-        lines.append(f"rng.state={rng_state}")
+    lines += [f"{k}={v}" for k, v in (("rng.state", state.rng_state), ("rng.seed", state.rng_seed)) if v is not None]
     lines += [f"{k}={v}" for k, v in optimizer.meta_pairs()]
     if schedule is not None:
         lines += [f"{k}={v}" for k, v in schedule_pairs(schedule)]
@@ -210,15 +218,17 @@ def read_meta(path: str, optimizer):
                                        _parse_f64(m, "scaler.backoff_factor"),
                                        _parse_usize(m, "scaler.growth_interval"),
                                        _parse_usize(m, "scaler.consecutive_ok"))
-    try:
-        rng = _parse_usize(m, "rng.state")
-    except CheckpointError:
-        rng = None
+    rng = []
+    for key in ("rng.state", "rng.seed"):
+        try:
+            rng.append(_parse_usize(m, key))
+        except CheckpointError:
+            rng.append(None)
     try:
         schedule = parse_schedule_state(m)
     except OptimStateError as e:
         raise CheckpointError("Optim", str(e)) from None
-    return scaler_state, TrainState(epoch, step, grad_accum, rng), schedule
+    return scaler_state, TrainState(epoch, step, grad_accum, *rng), schedule
 
 
 def _native(call, *args):

@@ -22,8 +22,8 @@ the two decisions stay separate entry points in the reference's order.
 
 A generator given with `with_rng` (nabla_amd.ops.DropoutRng) is advanced once per micro-batch,
 whatever became of it, so that the dropouts of the next one draw other masks; its step is
-`state.rng_state`, which checkpoints carry (checkpoint.rs:107-150, `rng.state`).  The device has the
-only copy: whatever else advances or loads the generator, a replayed graph among it, a checkpoint has
+`state.rng_state`, its seed `state.rng_seed`, and checkpoints carry both (checkpoint.rs:107-150, `rng.state`;
+`rng.seed` is a line of this library's own).  The device has the only copy: whatever else advances or loads the generator, a replayed graph among it, a checkpoint has
 the step that the next mask is drawn with.
 """
 from __future__ import annotations
@@ -83,7 +83,8 @@ class TrainerTail:
 
     def with_rng(self, rng) -> "TrainerTail":
         """`rng`: the ops.DropoutRng whose step one micro-batch's forward and backward pass share.
-        Where a checkpoint has left a step in `state`, the generator goes on from there."""
+        Where a checkpoint has left its step and seed in `state`, the generator goes on from there; a file
+        without a seed (the reference's) leaves the generator its own."""
         self.rng = rng
         self._state.follow(rng)
         return self

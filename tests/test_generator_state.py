@@ -132,3 +132,66 @@ def test_checkpoint_after_replays_of_a_graph_that_advances_the_generator(gpu, tm
             assert torch.equal(y, z) and not torch.equal(last, y)
     finally:
         _lib.check(lib.nbo_set_stream(None))
+
+
+# ---- the seed ------------------------------------------------------------------------------
+
+
+def test_checkpoint_carries_the_seed(tmp_path):
+    """A run that is resumed with a generator of another seed draws the first one's masks."""
+    tail = tail_of(FakeRng((1 << 64) - 9, 100))
+    tail.after_backward([])
+    state = written(tmp_path, tail.state)
+    assert (state.rng_state, state.rng_seed) == (101, (1 << 64) - 9)
+    assert "rng.state=101\nrng.seed=18446744073709551607\n" in (tmp_path / "meta.txt").read_text()
+    for attach_first in (True, False):
+        rng = FakeRng(5, 0)
+        resumed = tail_of(rng) if attach_first else TrainerTail(FakeOptimizer(), [])
+        resumed.set_state(copy.copy(state))
+        resumed.with_rng(rng)
+        assert rng.at == ops.DropoutRngState((1 << 64) - 9, 101)
+        resumed.with_rng(FakeRng(6, 0))  # another generator on purpose: its own seed
+        assert resumed.state.rng_seed == 6 and resumed.state.rng_state == 101
+
+
+def test_checkpoints_without_a_seed_are_read_and_written_as_before(tmp_path):
+    state = written(tmp_path, ck.TrainState(1, 2, 3, 4))
+    assert state == ck.TrainState(1, 2, 3, 4) and state.rng_seed is None
+    assert "rng.seed" not in (tmp_path / "meta.txt").read_text()
+    rng = FakeRng(5, 0)
+    tail_of(rng).set_state(state)
+    assert rng.at == ops.DropoutRngState(5, 4)
+
+
+def test_cpp_side_reads_and_writes_the_seed(tmp_path):
+    import os
+    import subprocess
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "t.cpp"
+    src.write_text(r"""
+#include "nabla_checkpoint.hpp"
+using namespace nabla::optim;
+namespace nabla { namespace optim {
+struct Opt {}; // found by its namespace
+Pairs meta_pairs_of(const Opt &) { return {}; }
+void load_meta_pairs_into(Opt &, const MetaMap &) {}
+} }
+int main(int, char **argv)
+{
+    Opt o;
+    const MetaContents in = read_meta(argv[1], o);
+    write_meta(argv[2], o, nullptr, nullptr, in.state);
+    return 0;
+}
+""")
+    libdir = os.path.join(root, "nabla_amd")
+    r = subprocess.run(["g++", "-O0", "-std=c++17", "-Wall", "-Wextra", "-Werror", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                        "-I", os.path.join(root, "include"), "-o", str(tmp_path / "t"), str(src), "-L", libdir,
+                        "-l:libnabla_optim.so", f"-Wl,-rpath,{libdir}", "-Wl,-rpath,/opt/rocm/lib"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    for k, state in enumerate([ck.TrainState(1, 2, 3, 4, (1 << 64) - 9), ck.TrainState(1, 2, 3, 4), ck.TrainState(1, 2, 3)]):
+        written(tmp_path, state)
+        out = tmp_path / f"out{k}.txt"
+        assert subprocess.run([str(tmp_path / "t"), str(tmp_path / "meta.txt"), str(out)]).returncode == 0
+        assert out.read_text() == (tmp_path / "meta.txt").read_text()
