@@ -123,11 +123,8 @@ Runtime::Runtime()
              std::string("hipModuleLoadData of the embedded gfx950 code object failed: ") +
                  hipGetErrorString(e));
     }
-    hip_check(hipModuleLoadData(&ops_module_, nbo_ops_code_object), "hipModuleLoadData (operators)");
-    for (int k = 0; k < K_COUNT; k++)
-        if (kKernelNames[k])
-            hip_check(hipModuleGetFunction(&fn_[k], k < K_OPS_BASE ? module_ : ops_module_, kKernelNames[k]),
-                      kKernelNames[k]);
+    for (int k = 0; k < K_OPS_BASE; k++)
+        if (kKernelNames[k]) hip_check(hipModuleGetFunction(&fn_[k], module_, kKernelNames[k]), kKernelNames[k]);
     pinned_bytes_ = 8 << 20; // two halves of 4 MiB
     hip_check(hipHostMalloc(&pinned_, pinned_bytes_, hipHostMallocDefault), "hipHostMalloc");
     for (hipEvent_t &e : staged_) hip_check(hipEventCreateWithFlags(&e, hipEventDisableTiming), "hipEventCreate");
@@ -169,8 +166,30 @@ void Runtime::set_stream(hipStream_t s)
     stream_ = s;
 }
 
-hipFunction_t Runtime::function(int kernel) const
+void Runtime::load_operators()
 {
+    if (ops_module_) return;
+    // The first operator may be a call that a graph captures: nothing here is part of the graph.
+    struct Relaxed {
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        Relaxed() { hip_check(hipThreadExchangeStreamCaptureMode(&mode), "hipThreadExchangeStreamCaptureMode"); }
+        ~Relaxed() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    } relaxed;
+    hipModule_t m = nullptr;
+    hip_check(hipModuleLoadData(&m, nbo_ops_code_object), "hipModuleLoadData (operators)");
+    try {
+        for (int k = K_OPS_BASE; k < K_COUNT; k++)
+            hip_check(hipModuleGetFunction(&fn_[k], m, kKernelNames[k]), kKernelNames[k]);
+    } catch (...) {
+        (void)hipModuleUnload(m);
+        throw;
+    }
+    ops_module_ = m;
+}
+
+hipFunction_t Runtime::function(int kernel)
+{
+    if (kernel >= K_OPS_BASE && kernel < K_COUNT) load_operators();
     if (kernel >= 0 && kernel < K_COUNT && fn_[kernel]) return fn_[kernel];
     if (kernel >= K_COUNT && (size_t)(kernel - K_COUNT) < bench_fn_.size()) return bench_fn_[kernel - K_COUNT];
     fail(NBO_ERR_ARG, "internal: unknown kernel id " + std::to_string(kernel));

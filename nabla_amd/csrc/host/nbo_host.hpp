@@ -126,6 +126,9 @@ public:
     // loaded when the first such id is asked for; the id works with launch, time_launches and
     // the per-kernel timing like the ids above.
     int bench_kernel(const char *name);
+    // The code object of the operators (nbo_ops_kernels.hip), which a process that only steps an optimizer does not
+    // load: their handles ask for it, and otherwise the first launch.
+    void load_operators();
     void launch_copy(const void *src, void *dst, uint64_t nvec);
     // float i of the nvec 128-bit vectors at dst = i mod 1024 (start contents of a checked probe run)
     void launch_fill_index(void *dst, uint64_t nvec);
@@ -166,10 +169,10 @@ public:
 
 private:
     Runtime();
-    hipFunction_t function(int kernel) const;
+    hipFunction_t function(int kernel);
     const char *kernel_name(int kernel) const;
     hipModule_t module_ = nullptr;
-    hipModule_t ops_module_ = nullptr;
+    hipModule_t ops_module_ = nullptr; // loaded on first use
     hipFunction_t fn_[K_COUNT] = {};
     uint32_t grid_x_max_ = 0xFFFFFFu;
     hipModule_t bench_module_ = nullptr; // loaded on first use

@@ -338,6 +338,7 @@ int nbo_embedding_ws_create(uint64_t max_ids, uint64_t max_cols, nbo_embedding_w
         require(max_ids <= MAX_ROWS && max_cols <= MAX_COLS, NBO_ERR_TOO_LARGE, "more than 2^31 - 2 ids or 2^27 columns");
         Runtime &rt = Runtime::get();
         const OnDevice on(rt.device());
+        rt.load_operators();
         nbo_embedding_ws *w = new nbo_embedding_ws();
         try {
             w->max_ids = max_ids;
@@ -476,6 +477,7 @@ int nbo_rng_create(uint64_t seed, uint64_t step, nbo_rng **out)
         *out = nullptr;
         Runtime &rt = Runtime::get();
         const OnDevice on(rt.device());
+        rt.load_operators();
         nbo_rng *r = new nbo_rng();
         try {
             r->dev = (NboRngDev *)rt.dmalloc(sizeof(NboRngDev));

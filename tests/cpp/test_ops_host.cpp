@@ -1,0 +1,86 @@
+// The host side of the operators (nbo_ops.cpp) without a GPU, over a HIP runtime that notes what it is asked
+// for.  One test to a run: `test_ops_host.bin NAME`; exit code 0 = passed.
+#include "hip_stub.hpp"
+
+#include <cstdio>
+
+#include "../../include/nabla_ops.h"
+
+static int failures = 0;
+#define EXPECT(cond)                                                        \
+    do {                                                                    \
+        if (!(cond)) {                                                      \
+            std::printf("  FAILED %s:%d: %s\n", __FILE__, __LINE__, #cond); \
+            failures++;                                                     \
+        }                                                                   \
+    } while (0)
+
+namespace {
+void *device(size_t bytes)
+{
+    void *p = nullptr;
+    (void)hipMalloc(&p, bytes);
+    return p;
+}
+nbo_matrix matrix(uint64_t rows, uint64_t cols, int dtype)
+{
+    return nbo_matrix{device(rows * cols * (dtype == NBO_DT_F64 ? 8 : dtype == NBO_DT_F32 ? 4 : 2)), rows, cols, cols, dtype, 0};
+}
+nbo_ids ids_of(uint64_t n) { return nbo_ids{device(n * 8), n, NBO_ID_I64, 0}; }
+
+int lookup()
+{
+    const nbo_matrix table = matrix(9, 16, NBO_DT_F32), out = matrix(3, 16, NBO_DT_F32);
+    const nbo_ids ids = ids_of(3);
+    return nbo_embedding(&table, &ids, nullptr, 1.0, &out);
+}
+
+// A process that clears gradients (or steps an optimizer) loads one code object; the operators' comes
+// with the first of them, inside a capture too.
+void loads_the_operators_when_they_are_used()
+{
+    EXPECT(nbo_init() == NBO_OK);
+    const uint64_t rows = 4, cols = 8;
+    void *g = device(rows * cols * 4);
+    nbo_list *list = nullptr;
+    EXPECT(nbo_list_create(1, &rows, &cols, NBO_DT_F32, &g, &list) == NBO_OK);
+    EXPECT(nbo_zero_grad(list) == NBO_OK);
+    EXPECT(stub::modules.size() == 1);
+    EXPECT(lookup() == NBO_OK);
+    EXPECT(stub::modules.size() == 2 && stub::load_mode == hipStreamCaptureModeRelaxed &&
+           stub::capture_mode == hipStreamCaptureModeGlobal);
+    EXPECT(lookup() == NBO_OK);
+    EXPECT(stub::modules.size() == 2);
+}
+void handles_load_the_operators()
+{
+    nbo_rng *rng = nullptr;
+    EXPECT(nbo_rng_create(1, 2, &rng) == NBO_OK);
+    EXPECT(stub::modules.size() == 2);
+}
+// An operators' code object that does not load takes nothing else with it, and is tried again.
+void optimizers_do_without_the_operators()
+{
+    stub::fail_module = 1;
+    EXPECT(nbo_init() == NBO_OK);
+    EXPECT(lookup() == NBO_ERR_HIP + (int)hipErrorNoBinaryForGpu);
+    EXPECT(stub::capture_mode == hipStreamCaptureModeGlobal);
+    EXPECT(lookup() == NBO_OK);
+}
+} // namespace
+
+int main(int argc, char **argv)
+{
+    const std::map<std::string, void (*)()> tests = {
+        {"loads_the_operators_when_they_are_used", loads_the_operators_when_they_are_used},
+        {"handles_load_the_operators", handles_load_the_operators},
+        {"optimizers_do_without_the_operators", optimizers_do_without_the_operators},
+    };
+    if (argc < 2) {
+        for (const auto &t : tests) std::printf("%s\n", t.first.c_str());
+        return 0;
+    }
+    tests.at(argv[1])();
+    std::printf("%d failure(s)\n", failures);
+    return failures ? 1 : 0;
+}
