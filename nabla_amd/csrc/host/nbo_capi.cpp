@@ -34,18 +34,20 @@ bool pointer_checks_enabled()
     return on;
 }
 
-void check_device_address(const void *ptr, uint64_t bytes, const char *what, int device)
+void check_device_address(const void *ptr, uint64_t bytes, const char *what, int device, int64_t number)
 {
-    char where[96];
-    std::snprintf(where, sizeof(where), "%s at %p", what, ptr);
+    auto refuse = [&](const std::string &why) { // (the text costs more than the checks)
+        char at[32];
+        std::snprintf(at, sizeof(at), " at %p", ptr);
+        fail(NBO_ERR_ARG, what + (number >= 0 ? " " + std::to_string(number) : std::string()) + at + ": " + why);
+    };
     hipPointerAttribute_t attr;
     const hipError_t e = hipPointerGetAttributes(&attr, ptr);
     if (e != hipSuccess) (void)hipGetLastError();
     if (e != hipSuccess || attr.type == hipMemoryTypeUnregistered)
-        fail(NBO_ERR_ARG, std::string(where) + ": not memory the HIP runtime knows (a host pointer?)");
+        refuse("not memory the HIP runtime knows (a host pointer?)");
     if (device >= 0 && attr.type == hipMemoryTypeDevice && attr.device != device)
-        fail(NBO_ERR_ARG, std::string(where) + ": memory of device " + std::to_string(attr.device) +
-                              ", the library works on device " + std::to_string(device));
+        refuse("memory of device " + std::to_string(attr.device) + ", the library works on device " + std::to_string(device));
     hipDeviceptr_t base = nullptr;
     size_t size = 0;
     if (hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)ptr) != hipSuccess) {
@@ -54,8 +56,7 @@ void check_device_address(const void *ptr, uint64_t bytes, const char *what, int
     }
     const uintptr_t end = (uintptr_t)base + size, p = (uintptr_t)ptr;
     if (p < (uintptr_t)base || bytes > end - p)
-        fail(NBO_ERR_ARG, std::string(where) + ": " + std::to_string(bytes) + " bytes do not fit the allocation (" +
-                              std::to_string(end - p) + " bytes from there to its end)");
+        refuse(std::to_string(bytes) + " bytes do not fit the allocation (" + std::to_string(end - p) + " bytes from there to its end)");
 }
 
 } // namespace nbo
@@ -381,9 +382,7 @@ uint32_t state_part_index(const nbo_optim *opt, char which)
 
 void check_tensor_address(const void *ptr, uint64_t bytes, uint64_t t)
 {
-    char what[32];
-    std::snprintf(what, sizeof(what), "tensor %llu", (unsigned long long)t);
-    check_device_address(ptr, bytes, what);
+    check_device_address(ptr, bytes, "tensor", -1, (int64_t)t);
 }
 
 // Copies the n elements of tensor i's part `part` between the arena and a dense

@@ -266,10 +266,10 @@ struct nbo_placed {
 
 namespace nbo {
 // Address checks (nbo_capi.cpp): whether they are on, and NBO_ERR_ARG unless `bytes` bytes at ptr lie in
-// memory the HIP runtime knows -- with `device` >= 0, not in another device's; `what` names the tensor in
-// the message.
+// memory the HIP runtime knows -- with `device` >= 0, not in another device's; `what` (and, with >= 0, `number`)
+// names the tensor in the message.
 bool pointer_checks_enabled();
-void check_device_address(const void *ptr, uint64_t bytes, const char *what, int device = -1);
+void check_device_address(const void *ptr, uint64_t bytes, const char *what, int device, int64_t number = -1);
 
 // NBLA tensor files (nbo_nbla.cpp)
 void nbla_save_list(const char *path, const nbo_list *list, const char *const *names);

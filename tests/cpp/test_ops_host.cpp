@@ -67,11 +67,40 @@ void optimizers_do_without_the_operators()
     EXPECT(stub::capture_mode == hipStreamCaptureModeGlobal);
     EXPECT(lookup() == NBO_OK);
 }
+// Which tensor it was, and where.
+std::string at(const void *p)
+{
+    char text[32];
+    std::snprintf(text, sizeof(text), " at %p: ", p);
+    return text;
+}
+void addresses_are_named()
+{
+    EXPECT(nbo_init() == NBO_OK);
+    const uint64_t rows[2] = {4, 4}, cols[2] = {8, 8};
+    float host[32];
+    void *good = device(128), *ptrs[2] = {good, host};
+    nbo_list *list = nullptr;
+    EXPECT(nbo_list_create(2, rows, cols, NBO_DT_F32, ptrs, &list) == NBO_ERR_ARG);
+    EXPECT(nbo_last_error() == "tensor 1" + at(host) + "not memory the HIP runtime knows (a host pointer?)");
+    ptrs[1] = (char *)good + 4;
+    EXPECT(nbo_list_create(2, rows, cols, NBO_DT_F32, ptrs, &list) == NBO_ERR_ARG);
+    EXPECT(nbo_last_error() == "tensor 1" + at(ptrs[1]) + "128 bytes do not fit the allocation (124 bytes from there to its end)");
+    const nbo_matrix table = matrix(9, 16, NBO_DT_F32), out = matrix(3, 16, NBO_DT_F32);
+    const nbo_ids ids = ids_of(3), beyond{ids.data, 4, NBO_ID_I64, 0}, on_host{host, 3, NBO_ID_I32, 0};
+    nbo_matrix more = out;
+    more.rows = 4;
+    EXPECT(nbo_embedding(&table, &beyond, nullptr, 1.0, &more) == NBO_ERR_ARG);
+    EXPECT(nbo_last_error() == "ids" + at(ids.data) + "32 bytes do not fit the allocation (24 bytes from there to its end)");
+    EXPECT(nbo_embedding(&table, &on_host, nullptr, 1.0, &out) == NBO_ERR_ARG);
+    EXPECT(nbo_last_error() == "ids" + at(host) + "not memory the HIP runtime knows (a host pointer?)");
+}
 } // namespace
 
 int main(int argc, char **argv)
 {
     const std::map<std::string, void (*)()> tests = {
+        {"addresses_are_named", addresses_are_named},
         {"loads_the_operators_when_they_are_used", loads_the_operators_when_they_are_used},
         {"handles_load_the_operators", handles_load_the_operators},
         {"optimizers_do_without_the_operators", optimizers_do_without_the_operators},

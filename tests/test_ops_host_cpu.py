@@ -5,7 +5,7 @@ import subprocess
 import pytest
 
 BIN = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "test_ops_host.bin")
-NAMES = ["handles_load_the_operators", "loads_the_operators_when_they_are_used", "optimizers_do_without_the_operators"]
+NAMES = ["addresses_are_named", "handles_load_the_operators", "loads_the_operators_when_they_are_used", "optimizers_do_without_the_operators"]
 
 
 def test_all_are_run():
