@@ -8,7 +8,8 @@
  * function returns an nbo_status and leaves a message for nbo_last_error(), nothing throws, all
  * work is enqueued on the library's stream (nbo_set_stream) on device 0 in call order, and what
  * returns nothing to the host does not synchronise.  The operators themselves allocate nothing and
- * may be captured into a HIP graph; their handles are created beforehand.
+ * may be captured into a HIP graph; their handles are created beforehand, and they and the tensors
+ * stay for as long as the graph is replayed.
  */
 #ifndef NABLA_OPS_H
 #define NABLA_OPS_H
@@ -88,10 +89,10 @@ int nbo_rng_advance(nbo_rng *rng, uint64_t steps); /* step += steps (modulo 2^64
  * Element e = row * cols + col is dropped if its 16 bits of Philox4x32-10 are below thr: key = seed;
  * counter = (e / 8, site, step's low half, step's high half); the bits are half e % 2 (low first) of
  * word e % 8 / 2.  `site` tells the dropouts of one step apart (one number per place in the model).  A
- * dropped element is zero whatever x holds there (inf, NaN).  The gradient is the same call on the gradient, without residual, at the
- * same seed, step and site.  Computed in f32 (f64: f64), rounded once.  x, residual and out have one
- * shape and type; out may be x or residual itself, other overlaps are NBO_ERR_ARG.  At most 2^35
- * elements.  Asynchronous. */
+ * dropped element is zero whatever x holds there (inf, NaN).  The gradient is the same call on the
+ * gradient, without residual, at the same seed, step and site.  Computed in f32 (f64: f64), rounded
+ * once.  x, residual and out have one shape and type; out may be x or residual itself, other overlaps
+ * are NBO_ERR_ARG.  At most 2^35 elements.  Asynchronous. */
 int nbo_dropout(const nbo_matrix *x, const nbo_matrix *residual, double p, nbo_rng *rng, uint32_t site,
                 const nbo_matrix *out);
 

@@ -21,6 +21,12 @@ stream, nothing allocated, nothing read back, so that a call may be captured int
 Tensors are torch tensors on cuda:0, or anything else with ``data_ptr()``, ``shape`` and
 ``dtype``.  A tensor of more than two dimensions stands for the matrix of its last one; rows may be
 strided, the elements of a row are adjacent.
+
+The calls are outside torch's autograd, as the optimizers' are: what they write has no graph behind it, and the
+backward pass calls ``dropout_grad`` and ``embedding_grad`` itself.  So a tensor that requires a gradient is
+refused where gradients are recorded (``detach()`` it, or call under ``torch.no_grad()``, as inside a
+``torch.autograd.Function``), and autograd is told that the tensor a call has written holds other values.
+A graph that has captured a call needs its tensors, workspace and generator for as long as it is replayed.
 """
 from __future__ import annotations
 
@@ -31,11 +37,20 @@ from typing import Optional
 from . import _lib
 from .optim import _call, _dtype_code, _shape2
 
+try:
+    from torch import Tensor as _Tensor, is_grad_enabled as _recording
+    from torch.autograd.graph import increment_version as _increment_version
+except ImportError:  # other tensors have no autograd
+    _Tensor = _recording = _increment_version = None
+
 
 _dtype_codes = {}  # by dtype object: spares the smallest calls the name's parsing
 
 
 def _matrix(t) -> _lib.Matrix:
+    if getattr(t, "requires_grad", False) and _recording is not None and _recording():
+        raise RuntimeError("this call is not recorded by autograd, and a tensor given to it requires a gradient: pass "
+                           "tensor.detach() or call under torch.no_grad()")
     try:
         rows, cols = t.shape
         stride, unit = t.stride()
@@ -49,7 +64,15 @@ def _matrix(t) -> _lib.Matrix:
     code = _dtype_codes.get(t.dtype)
     if code is None:
         code = _dtype_codes[t.dtype] = _dtype_code(t)
-    return _lib.Matrix(t.data_ptr(), rows, cols, stride, code, 0)
+    return _lib.Matrix(t.data_ptr(), rows, cols, stride, code)
+
+
+def _done(status: int, written) -> None:
+    """The end of a call that has written a tensor: what autograd has saved of it for a backward pass is gone."""
+    if status:
+        _call(status)
+    if _Tensor is not None and isinstance(written, _Tensor):
+        _increment_version(written)
 
 
 _id_codes = {}
@@ -64,8 +87,10 @@ def _ids(t) -> _lib.Ids:
         code = _id_codes[t.dtype] = _lib.ID_I64 if name == "int64" else _lib.ID_I32
     if hasattr(t, "is_contiguous") and not t.is_contiguous():
         raise ValueError("ids must be contiguous")
-    rows, cols = _shape2(t)
-    return _lib.Ids(t.data_ptr(), rows * cols, code, 0)
+    n = 1
+    for k in t.shape:
+        n *= int(k)
+    return _lib.Ids(t.data_ptr(), n, code)
 
 
 def embedding(table, ids, out, scale: float = 1.0, add=None) -> None:
@@ -75,7 +100,7 @@ def embedding(table, ids, out, scale: float = 1.0, add=None) -> None:
     `out` has the table's type, or bf16 / f16 over an f32 table; `add` has out's type and may be
     `out` itself.  Computed in f32 (f64 tables: f64), rounded once."""
     a = _matrix(add) if add is not None else None
-    _call(_lib.load().nbo_embedding(_matrix(table), _ids(ids), a, scale, _matrix(out)))
+    _done(_lib.load().nbo_embedding(_matrix(table), _ids(ids), a, scale, _matrix(out)), out)
 
 
 class EmbeddingWorkspace:
@@ -107,8 +132,8 @@ def embedding_grad(grad_out, ids, grad, workspace: EmbeddingWorkspace, scale: fl
     rows no id names are not touched.  What rows of `grad_out` hold whose id is outside the table does
     not matter.  `grad` has grad_out's type, or f32 under bf16 / f16.  Sums are f32 (f64: f64) in a fixed
     order, the same bits on every run, rounded once."""
-    _call(_lib.load().nbo_embedding_grad(_matrix(grad_out), _ids(ids), scale, 1 if accumulate else 0, _matrix(grad),
-                                         workspace._h))
+    _done(_lib.load().nbo_embedding_grad(_matrix(grad_out), _ids(ids), scale, 1 if accumulate else 0, _matrix(grad),
+                                         workspace._h), grad)
 
 
 @dataclass
@@ -164,7 +189,7 @@ def dropout(x, p: float, rng: DropoutRng, site: int, out, residual=None) -> None
     if not 0 <= site < 1 << 32:
         raise ValueError(f"site {site} is not an unsigned 32-bit number")
     r = _matrix(residual) if residual is not None else None
-    _call(_lib.load().nbo_dropout(_matrix(x), r, p, rng._h, site, _matrix(out)))
+    _done(_lib.load().nbo_dropout(_matrix(x), r, p, rng._h, site, _matrix(out)), out)
 
 
 def dropout_grad(grad_out, p: float, rng: DropoutRng, site: int, out) -> None:
