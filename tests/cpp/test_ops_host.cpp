@@ -5,6 +5,7 @@
 #include <cstdio>
 
 #include "../../include/nabla_ops.h"
+#include "../../nabla_amd/csrc/nbo_ops_types.h"
 
 static int failures = 0;
 #define EXPECT(cond)                                                        \
@@ -95,6 +96,37 @@ void addresses_are_named()
     EXPECT(nbo_embedding(&table, &on_host, nullptr, 1.0, &out) == NBO_ERR_ARG);
     EXPECT(nbo_last_error() == "ids" + at(host) + "not memory the HIP runtime knows (a host pointer?)");
 }
+
+// What runs for a gradient: `test_ops_host.bin plan IDS ROWS COLS TYPE GRAD_TYPE ACCUMULATE`, a launch to a line.
+int plan(char **argv)
+{
+    auto number = [&](int k) { return std::strtoull(argv[k], nullptr, 10); };
+    stub::args_bytes = [](const std::string &name) -> size_t {
+        return name.compare(0, 14, "nbo_embed_sum_") == 0 || name.compare(0, 15, "nbo_embed_join_") == 0 ? sizeof(NboEmbedGradArgs)
+               : name.compare(0, 10, "nbo_order_") == 0                                                   ? sizeof(NboOrderArgs)
+                                                                                                          : 0;
+    };
+    const nbo_ids ids = ids_of(number(2));
+    const nbo_matrix dy = matrix(ids.n, number(4), (int)number(5)), grad = matrix(number(3), number(4), (int)number(6));
+    nbo_embedding_ws *ws = nullptr;
+    EXPECT(nbo_embedding_ws_create(ids.n, grad.cols, &ws) == NBO_OK);
+    stub::launches.clear();
+    EXPECT(nbo_embedding_grad(&dy, &ids, 1.0, (int)number(7), &grad, ws) == NBO_OK);
+    for (const stub::Launch &l : stub::launches) {
+        std::printf("%s grid %u %u", l.name.c_str(), l.gx, l.gy);
+        if (l.args.size() == sizeof(NboEmbedGradArgs)) {
+            NboEmbedGradArgs a;
+            std::memcpy((void *)&a, l.args.data(), sizeof(a));
+            std::printf(" piece %u pieces %u lanes %u slabs %u edges %u", a.piece, a.pieces, a.lanes, a.slabs, a.edges);
+        } else if (l.args.size() == sizeof(NboOrderArgs)) {
+            NboOrderArgs a;
+            std::memcpy((void *)&a, l.args.data(), sizeof(a));
+            std::printf(" tiles %u digits %u range %u", a.tiles, a.digits, a.range);
+        }
+        std::printf("\n");
+    }
+    return failures;
+}
 } // namespace
 
 int main(int argc, char **argv)
@@ -109,6 +141,7 @@ int main(int argc, char **argv)
         for (const auto &t : tests) std::printf("%s\n", t.first.c_str());
         return 0;
     }
+    if (argc == 8 && argv[1] == std::string("plan")) return plan(argv);
     tests.at(argv[1])();
     std::printf("%d failure(s)\n", failures);
     return failures ? 1 : 0;

@@ -4,6 +4,11 @@ import subprocess
 import sys
 
 import pytest
+import torch
+
+from nabla_amd import _lib, ops
+from nabla_amd import optim as nb
+from tests.test_gpu_ops import DEV, kept, rand_ids, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +43,170 @@ print("captured ok")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100, cwd=ROOT,
                        env=dict(os.environ, PYTHONPATH=ROOT))
     assert r.returncode == 0 and "captured ok" in r.stdout, r.stdout[-2000:] + r.stderr[-3000:]
+
+
+# ---- a training step, by each of the gradient's ways ------------------------------------------
+
+# (sequences, their length, rows of the token table): what runs between the ids and the gradient
+WAYS = {
+    "direct": (3, 130, 700, ["nbo_embed_direct_f32"]),
+    "range": (3, 500, 700, ["nbo_order_range", "nbo_embed_sum_f32", "nbo_embed_join_f32"]),
+    "split": (3, 3000, 700, ["nbo_order_split", "nbo_order_merge", "nbo_embed_sum_f32", "nbo_embed_join_f32"]),
+    "radix": (3, 3000, 530_000, ["nbo_order_hist", "nbo_order_scan", "nbo_order_scatter", "nbo_embed_sum_f32",
+                                 "nbo_embed_join_f32"]),
+}
+
+
+class Block:
+    """dropout(2 wte[tokens] + wpe[positions]) and its gradients, next to an AdamW over both tables."""
+
+    def __init__(self, seed, way):
+        self.batch, self.seq, self.rows, self.kernels = WAYS[way]
+        self.cols, self.n = 136, self.batch * self.seq
+        self.params = [randn(self.rows, self.cols, "f32", seed), randn(self.seq, self.cols, "f32", seed + 1)]
+        self.grads = [torch.zeros_like(p) for p in self.params]
+        self.tokens = rand_ids(self.n, self.rows, seed + 2, 0.1, True).reshape(self.batch, self.seq)
+        self.positions = torch.arange(self.seq, device=DEV, dtype=torch.int32).repeat(self.batch)
+        self.target = randn(self.n, self.cols, "f32", seed + 3)
+        self.x, self.dx = torch.empty_like(self.target), torch.empty_like(self.target)
+        self.ws = ops.EmbeddingWorkspace(self.n, self.cols)
+        self.rng = ops.DropoutRng(seed, 17)
+        self.opt = nb.AdamW.new(1e-2, [tuple(p.shape) for p in self.params])
+        self.plist, self.glist = nb.TensorList(self.params), nb.TensorList(self.grads)
+        self.tokens_grad = nb.TensorList(self.grads[:1])
+
+    def gradients(self):
+        ops.embedding(self.params[1], self.positions, self.x)
+        ops.embedding(self.params[0], self.tokens, self.x, scale=2.0, add=self.x)
+        ops.dropout(self.x, 0.2, self.rng, 4, self.x)
+        torch.sub(self.x, self.target, out=self.dx)  # d/dx of half the squared distance
+        ops.dropout_grad(self.dx, 0.2, self.rng, 4, self.dx)
+        ops.embedding_grad(self.dx, self.positions, self.grads[1], self.ws)  # fresh: the positions' table is cleared
+        ops.embedding_grad(self.dx, self.tokens, self.grads[0], self.ws, scale=2.0, accumulate=True)
+        self.rng.advance()
+
+    def step(self):
+        self.gradients()
+        self.opt.step(self.plist, self.glist)  # (no norm pass: its scratch is one for the whole library)
+        nb.zero_grad(self.tokens_grad)
+
+    def state(self):
+        return [self.x, self.dx] + self.grads + self.params + [self.opt.read_state(k) for k in ("m0", "v0", "m1", "v1")]
+
+
+def launched(kernels, call):
+    """How often each kernel runs in call()."""
+    import ctypes as C
+
+    lib, counts = _lib.load(), {}
+    _lib.check(lib.nbo_profile_enable(1))
+    try:
+        call()
+        for k in kernels:
+            n, ms = C.c_uint64(0), C.c_double(0)
+            _lib.check(lib.nbo_profile_read(k.encode(), C.byref(n), C.byref(ms)))
+            counts[k] = n.value
+    finally:
+        _lib.check(lib.nbo_profile_enable(0))
+    return counts
+
+
+@pytest.mark.parametrize("way", list(WAYS))
+def test_gradients_of_the_input_block_against_autograd(gpu, way):
+    """One step's gradients against torch's autograd in f64 on the CPU."""
+    b = Block(5, way)
+    wte, wpe = (p.double().cpu().requires_grad_() for p in b.params)
+    keep, thr = kept(b.n * b.cols, 5, 17, 4, 0.2)
+    factor = keep.reshape(b.n, b.cols).cpu().double() * (65536.0 / (65536 - thr))
+    ids = b.tokens.reshape(-1).cpu()
+    ok = (ids >= 0) & (ids < b.rows)
+    rows, at = ids.clamp(0, b.rows - 1), b.positions.long().cpu()
+    twice, target = 2.0 * ok.double()[:, None], b.target.cpu().double()
+    y = (wpe[at] + twice * wte[rows]) * factor
+    (0.5 * (y - target) ** 2).sum().backward()
+    counts = launched(b.kernels, b.gradients)
+    assert all(counts.values()), counts
+    assert b.rng.state().step == 18
+    with torch.no_grad():  # what a term's roundings, some ten, are relative to
+        size = factor * (factor * (wpe[at].abs() + twice * wte[rows].abs()) + target.abs())
+    for got, want, where, scale in ((b.grads[0], wte.grad, rows, twice), (b.grads[1], wpe.grad, at, torch.ones_like(twice))):
+        terms = torch.zeros(len(want), 1, dtype=torch.float64).index_add_(0, where, scale.clamp(max=1.0))
+        bound = (terms + 10) * 2.0 ** -24 * (1 + 2 ** -10) * torch.zeros_like(want).index_add_(0, where, scale * size)
+        assert ((got.double().cpu() - want).abs() <= bound).all()
+        assert ((got.cpu() != 0) == (want != 0)).all()
+
+
+@pytest.mark.parametrize("ways", [("direct", "direct"), ("range", "range"), ("split", "split"), ("range", "split"),
+                                  ("radix", "split")], ids="-".join)
+def test_training_steps_replay_from_two_graphs_on_two_streams(gpu, ways):
+    """Forward, backward, optimizer step and the generator's advance, captured once: every replay is an eager
+    step of a twin, bit for bit.  Two graphs, each with its own workspace, are replayed at the same time."""
+    lib = _lib.load()
+    twins = [Block(5, ways[0]), Block(6, ways[1])]
+    blocks = [Block(5, ways[0]), Block(6, ways[1])]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs = []
+    torch.cuda.synchronize()
+    try:
+        for b, s in zip(blocks, streams):
+            _lib.check(lib.nbo_set_stream(s.cuda_stream))
+            with torch.cuda.stream(s):
+                b.step()
+                s.synchronize()
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=s):
+                    b.step()
+                s.synchronize()
+                graphs.append(g)
+    finally:
+        _lib.check(lib.nbo_set_stream(None))
+    torch.cuda.synchronize()
+    for t in twins:
+        counts = launched(t.kernels, t.step)
+        assert all(counts.values()), counts
+    for replay in range(4):
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+                if replay % 2:
+                    s.synchronize()
+        for t in twins:  # eager work between and beside the replays
+            t.step()
+        torch.cuda.synchronize()
+        for b, t in zip(blocks, twins):
+            assert b.rng.state() == t.rng.state() and b.rng.state().step == 19 + replay
+            for k, (got, want) in enumerate(zip(b.state(), t.state())):
+                assert torch.equal(got, want), (replay, k)
+
+
+@pytest.mark.parametrize("way", list(WAYS))
+def test_training_goes_on_from_a_checkpoint(gpu, tmp_path, way):
+    """Three micro-batches through TrainerTail, saved after the first and resumed with fresh objects (the
+    generator with another seed): the same masks, gradients and parameters."""
+    from nabla_amd import checkpoint as ck
+    from nabla_amd.trainer import TrainerTail
+
+    def micro_batch(b, tail):
+        ops.embedding(b.params[0], b.tokens, b.x)
+        ops.dropout(b.x, 0.3, b.rng, 2, b.x)
+        torch.sub(b.x, b.target, out=b.dx)
+        ops.dropout_grad(b.dx, 0.3, b.rng, 2, b.dx)
+        ops.embedding_grad(b.dx, b.tokens, b.grads[0], b.ws)
+        tail.after_backward(b.grads)
+
+    a = Block(5, way)
+    ta = TrainerTail(a.opt, a.params).with_rng(a.rng).with_grad_clip(1.0)
+    micro_batch(a, ta)
+    names = ["wte", "wpe"]
+    ck.save_checkpoint(str(tmp_path), list(zip(names, a.params)), a.opt, None, None, ta.state, native=True)
+    b = Block(5, way)
+    _, state, _ = ck.load_checkpoint(str(tmp_path), b.opt, into=list(zip(names, b.params)))
+    b.rng = ops.DropoutRng(99, 0)
+    tb = TrainerTail(b.opt, b.params).with_rng(b.rng).with_grad_clip(1.0)
+    tb.set_state(state)
+    for _ in range(2):
+        micro_batch(a, ta)
+        micro_batch(b, tb)
+        assert torch.equal(a.x, b.x) and a.rng.state() == b.rng.state()
+        assert torch.equal(a.params[0], b.params[0]) and torch.equal(a.grads[0], b.grads[0])
