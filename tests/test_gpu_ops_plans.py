@@ -8,7 +8,7 @@ import torch
 
 from nabla_amd import _lib, ops
 from nabla_amd import optim as nb
-from tests.test_gpu_ops import DEV, kept, rand_ids, randn
+from tests.test_gpu_ops import DEV, assert_within, check_grad, kept, rand_ids, randn, rounding
 
 pytestmark = pytest.mark.gpu
 
@@ -210,3 +210,77 @@ def test_training_goes_on_from_a_checkpoint(gpu, tmp_path, way):
         micro_batch(b, tb)
         assert torch.equal(a.x, b.x) and a.rng.state() == b.rng.state()
         assert torch.equal(a.params[0], b.params[0]) and torch.equal(a.grads[0], b.grads[0])
+
+
+# ---- pieces of every length, many boundaries, many tiles ---------------------------------------
+
+# (ids, rows, columns, types, hot ids, padding) and what the plan makes of them: (ids per piece, lanes that work on
+# one, waves side by side, boundaries to a workgroup of the join)
+PIECES = [
+    ((65537, 300, 2056, "f16", "f16", False, 0.0), (64, 64, 5, 2)),
+    ((65537, 3000, 2056, "bf16", "f32", True, 0.1), (64, 64, 5, 2)),
+    ((65537, 2000, 1030, "f64", "f64", True, 0.0), (64, 64, 9, 3)),
+    ((131073, 20000, 4104, "bf16", "bf16", True, 0.0), (64, 64, 9, 5)),
+    ((40001, 300, 2056, "bf16", "bf16", False, 0.0), (32, 64, 5, 2)),
+    ((40001, 9000, 2056, "f16", "f32", True, 0.2), (32, 64, 5, 2)),
+    ((20011, 900, 2056, "f32", "f32", True, 0.0), (32, 64, 9, 2)),
+    ((20011, 900, 2050, "bf16", "bf16", True, 0.1), (16, 64, 5, 2)),
+    ((600001, 3000, 200, "bf16", "bf16", True, 0.0), (64, 32, 1, 3)),
+    ((600001, 70000, 200, "f16", "f32", False, 0.1), (64, 32, 1, 3)),
+    ((300001, 3000, 200, "bf16", "bf16", True, 0.0), (32, 32, 1, 3)),
+    ((300001, 9000, 61, "f32", "f32", True, 0.3), (16, 16, 1, 5)),
+    ((1200001, 50000, 24, "bf16", "bf16", True, 0.0), (16, 4, 1, 19)),
+    ((17000001, 40000, 3, "f16", "f16", True, 0.0), (64, 1, 1, 64)),
+]
+
+
+def check_long_grad(dy, ids, grad, ws, scale, accumulate, what):
+    """check_grad with the sums of the definition on the CPU: on the GPU, torch's additions of a million f64 rows to
+    a few hot ones take seconds."""
+    rows, before = grad.shape[0], grad.clone()
+    at = torch.nonzero((ids >= 0) & (ids < rows))[:, 0]
+    i, x = ids[at].long().cpu(), dy[at].double().cpu()
+    total = torch.zeros(rows, grad.shape[1], dtype=torch.float64).index_add_(0, i, x).to(DEV)
+    size = torch.zeros(rows, grad.shape[1], dtype=torch.float64).index_add_(0, i, x.abs()).to(DEV)
+    m = torch.bincount(i, minlength=rows).double().to(DEV)[:, None]
+    want = scale * total + (before.double() if accumulate else 0.0)
+    ops.embedding_grad(dy, ids, grad, ws, scale=scale, accumulate=accumulate)
+    u, h, tiny = rounding(grad.dtype)
+    # m - 1 additions in some order, the factor and the product, the sum with what was there; the f64 sums' own
+    slack = ((m * u / (1 - m * u) + 3 * u + m * 2.0 ** -52) * abs(scale) * size + u * want.abs()) * (1 + 2 ** -20)
+    assert_within(grad, want, slack + h * (want.abs() + slack) + tiny, what)
+    rest = m[:, 0] == 0
+    assert torch.equal(grad[rest], before[rest] if accumulate else torch.zeros_like(before[rest])), what
+    first = grad.clone()
+    grad.copy_(before)
+    ops.embedding_grad(dy, ids, grad, ws, scale=scale, accumulate=accumulate)
+    assert torch.equal(first, grad), what + ": another run gives other bits"
+
+
+@pytest.mark.parametrize("case", [c for c, _ in PIECES], ids=lambda c: f"{c[0]}-{c[1]}x{c[2]}-{c[3]}-{c[4]}")
+def test_embedding_grad_over_whole_pieces(gpu, case):
+    """Tokens in every place of a piece: rows that fill it, begin and end in it, span many."""
+    n, rows, cols, dtype, gtype, hot, pad = case
+    ws = ops.EmbeddingWorkspace(n, cols)
+    ids = rand_ids(n, rows, 3, pad, hot)
+    dy = randn(n, cols, dtype, 1)
+    check = check_long_grad if n > 1 << 19 else check_grad
+    check(dy, ids, randn(rows, cols, gtype, 2), ws, 1.5, True, "accumulated")
+    ids[n // 3:n // 3 + 200] = rows - 1  # a row of some pieces beside the others
+    check(dy, ids, randn(rows, cols, gtype, 2), ws, 1.0, False, "fresh")
+
+
+# (ids, rows): radix passes over more tiles than a wave has lanes; tiles and passes
+TILES = [((300001, 600011), (74, 2)), ((530000, (1 << 21) + 5), (130, 3)), ((262145, 1 << 20), (65, 3))]
+
+
+@pytest.mark.parametrize("case", [c for c, _ in TILES], ids=lambda c: f"{c[0]}-{c[1]}")
+def test_embedding_grad_by_radix_passes_over_many_tiles(gpu, case):
+    n, rows = case
+    ws = ops.EmbeddingWorkspace(n, 4)
+    ids = rand_ids(n, rows, 3, 0.05)
+    ids[::7] = rows - 1
+    ids[3::11] = 0
+    check_long_grad(randn(n, 4, "f32", 1), ids, randn(rows, 4, "f32", 2), ws, 1.0, False, "fresh")
+    check_long_grad(randn(n, 3, "f16", 1), rand_ids(n, rows, 4, 0.1, True, torch.int32), randn(rows, 3, "f16", 2), ws, 1.0,
+                    True, "accumulated")
