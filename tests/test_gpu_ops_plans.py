@@ -284,3 +284,30 @@ def test_embedding_grad_by_radix_passes_over_many_tiles(gpu, case):
     check_long_grad(randn(n, 4, "f32", 1), ids, randn(rows, 4, "f32", 2), ws, 1.0, False, "fresh")
     check_long_grad(randn(n, 3, "f16", 1), rand_ids(n, rows, 4, 0.1, True, torch.int32), randn(rows, 3, "f16", 2), ws, 1.0,
                     True, "accumulated")
+
+
+# ---- the generator ----------------------------------------------------------------------------
+
+# counter, key and result of Philox4x32-10, as its authors publish them with their library (known answers)
+KNOWN = [((0, 0, 0, 0), (0, 0), (0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8)),
+         ((0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344), (0xa4093822, 0x299f31d0),
+          (0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1))]
+
+
+@pytest.mark.parametrize("known", KNOWN, ids=["zeros", "pi"])
+def test_known_answers_of_the_generator(gpu, known):
+    """Each 16 bits of the result from the masks: an element is kept at the rate that they are and dropped at the
+    next."""
+    (block, site, low, high), key, words = known
+    cols = 8 if block == 0 else 1 << 27
+    rows = block * 8 // cols + 1
+    if torch.cuda.mem_get_info(DEV)[0] < rows * cols * 4 + (1 << 30):
+        pytest.skip("needs 20 GB of free device memory")
+    x = torch.ones(rows, cols, device=DEV, dtype=torch.bfloat16)
+    out = torch.empty_like(x)
+    rng = ops.DropoutRng(key[0] | key[1] << 32, low | high << 32)
+    halves = [h for w in words for h in (w & 0xFFFF, w >> 16)]
+    for j, h in enumerate(halves):
+        for thr in (h, h + 1):
+            ops.dropout(x, thr / 65536, rng, site, out)
+            assert bool(out.reshape(-1)[block * 8 + j] != 0) == (h >= thr), (j, h, thr)
