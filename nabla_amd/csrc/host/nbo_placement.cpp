@@ -286,12 +286,15 @@ bool StatePlacement::try_placed(uint32_t nparts, size_t bytes, void **out, const
         for (uint32_t j = 0; j < nparts; j++)
             for (uint32_t k = j + 1; k < nparts; k++) {
                 if (pick_region[j][0] == pick_region[k][0]) continue;
-                const double g = rt.probe_pair_gbps(part_ranges[j].va, part_ranges[k].va, chunk);
+                const double thr = finder.threshold_between((size_t)pick_region[j][0], (size_t)pick_region[k][0]);
+                double g = 0.0;
+                const bool apart = plan::reads_apart(
+                    [&] { return rt.probe_pair_gbps(part_ranges[j].va, part_ranges[k].va, chunk); }, thr, &g);
                 if (debug > 1) std::fprintf(stderr, "[nbo placement] check, arrays %u and %u: %.0f GB/s\n", j, k, g);
-                if (!(g >= finder.threshold()))
+                if (!apart)
                     return fail_with(fmt("the finished layout did not check out: arrays %.0f and %.0f read %.0f GB/s together, "
                                          "below the threshold of %.0f",
-                                         (double)j, (double)k, g, finder.threshold()));
+                                         (double)j, (double)k, g, thr));
                 checked++;
             }
         success = true;

@@ -29,12 +29,15 @@ constexpr size_t kMaxRegions = 3;
 // (`same_pair`, its two halves, certainly of the low kind).  Anything else is scatter.
 constexpr double kMinClassRatio = 1.08;
 constexpr double kMinAboveSame = 1.03, kMaxAboveSame = 1.30;
+// What the "different" class is above a leader's two halves, at least, for these to be of one region.
+constexpr double kMinLeaderRatio = 1.05;
 
 // Threshold between "same region" and "different region" from measurements that all involve
 // one fixed chunk: the geometric mean of the two class means, or +infinity when the values do
 // not fall into two such classes (every value then reads "same").  No absolute bandwidth
 // enters, so a faster, slower or busier GPU moves both kinds together.
-inline double gap_threshold(std::vector<double> samples, double same_pair)
+// `upper`, if given, receives the mean of the "different" class.
+inline double gap_threshold(std::vector<double> samples, double same_pair, double *upper = nullptr)
 {
     const double inf = std::numeric_limits<double>::infinity();
     if (!(same_pair > 0.0)) return inf;
@@ -59,7 +62,20 @@ inline double gap_threshold(std::vector<double> samples, double same_pair)
     if (!(hi_mean >= lo_mean * kMinClassRatio)) return inf;
     const double thr = std::sqrt(lo_mean * hi_mean);
     if (thr < same_pair * kMinAboveSame || thr > same_pair * kMaxAboveSame) return inf;
+    if (upper) *upper = hi_mean;
     return thr;
+}
+
+// Whether two arrays read together at or above `threshold`: asked up to three times, because a probe that is
+// disturbed is slower, never faster.  `best` receives the fastest reading.
+template <typename Probe> bool reads_apart(Probe &&probe, double threshold, double *best)
+{
+    *best = 0.0;
+    for (int k = 0; k < 3 && !(*best >= threshold); k++) {
+        const double g = probe();
+        if (g > *best) *best = g;
+    }
+    return *best >= threshold;
 }
 
 // Sorts chunks into at most three regions.  Chunks arrive in rounds (add_chunks).  One chunk is
@@ -68,9 +84,13 @@ inline double gap_threshold(std::vector<double> samples, double same_pair)
 // halves (which certainly share a region).  Chunk 0 is the anchor unless its measurements show
 // no gap -- a chunk whose physical memory straddles two regions measures half-way against
 // everything -- in which case chunks 1 and 2 are tried.  Chunks that do not share the anchor's
-// region are measured against the first chunk of each further region ("leader") in turn.  A
-// chunk that differs from three leaders is left unused (region -1): a fourth kind can only be
-// noise.
+// region are measured against the first chunk of each further region ("leader") in turn, and each
+// leader has a threshold of its own: the regions differ in what two of their chunks measure together
+// (5.0-5.3 TB/s in one and 5.6 in another of the same process, with 5.61 as the anchor's threshold and 6.1
+// for chunks of both), so it lies between the leader's own two halves and the "different" class, and
+// not below the anchor's.  A leader whose halves come close to that class is pieced together and has
+// the anchor's.  A chunk that differs from three leaders is left unused (region -1): a fourth kind can
+// only be noise.
 class RegionFinder {
 public:
     static constexpr size_t kMaxAnchors = 3;
@@ -83,14 +103,16 @@ public:
         total_ = total;
         region_of_.assign(total_, -1);
         leaders_.clear();
+        thresholds_.clear();
         threshold_ = std::numeric_limits<double>::infinity();
+        double upper = 0.0;
         anchor_ = 0;
         if (total_ == 0) return;
         for (size_t a = 0; a < kMaxAnchors && a < total_; a++) {
             std::vector<double> v;
             for (size_t i = 0; i < total_; i++)
                 if (i != a) v.push_back(measure(a, i, probe));
-            const double t = gap_threshold(v, base_of(a, halves));
+            const double t = gap_threshold(v, base_of(a, halves), &upper);
             if (std::isfinite(t)) {
                 threshold_ = t;
                 anchor_ = a;
@@ -99,19 +121,24 @@ public:
             if (total_ < 4) break; // too few measurements to blame the anchor
         }
         leaders_.push_back(anchor_);
+        thresholds_.push_back(threshold_);
         for (size_t i = 0; i < total_; i++) {
             int region = -1;
             for (size_t k = 0; k < leaders_.size() && region < 0; k++)
-                if (measure(leaders_[k], i, probe) < threshold_) region = (int)k;
+                if (measure(leaders_[k], i, probe) < thresholds_[k]) region = (int)k;
             if (region < 0 && leaders_.size() < kMaxRegions) {
                 leaders_.push_back(i);
+                const double base = base_of(i, halves);
+                thresholds_.push_back(base * kMinLeaderRatio <= upper ? std::max(threshold_, std::sqrt(base * upper)) : threshold_);
                 region = (int)leaders_.size() - 1;
             }
             region_of_[i] = region;
         }
     }
 
-    double threshold() const { return threshold_; } // +infinity: no second region seen yet
+    double threshold() const { return threshold_; } // the anchor's; +infinity: no second region seen yet
+    // what chunks of two different regions read at least
+    double threshold_between(size_t a, size_t b) const { return std::max(thresholds_[a], thresholds_[b]); }
     double same_pair() const { return bases_.count(anchor_) ? bases_.at(anchor_) : 0.0; } // the anchor's halves
     size_t anchor() const { return anchor_; }
     size_t regions() const { return leaders_.size(); }
@@ -163,6 +190,7 @@ private:
     size_t total_ = 0, anchor_ = 0;
     std::vector<int> region_of_;
     std::vector<size_t> leaders_;
+    std::vector<double> thresholds_; // per region: below it a chunk shares the leader's
     std::map<std::pair<size_t, size_t>, double> cache_;
     std::map<size_t, double> bases_;
 };
