@@ -307,7 +307,8 @@ def flow_main(args) -> None:
 
 def ops_main(args) -> None:
     """The operators of nabla_ops.h (embedding lookup, its gradient, dropout) at the shapes of the
-    workloads: wall time of a call among others, and of each kernel it launches."""
+    workloads: wall time of a call among others, of each kernel it launches, and of PyTorch's own calls
+    for the same (F.embedding, the dense gradient that its backward pass makes, F.dropout)."""
     import time
 
     import torch
@@ -330,19 +331,28 @@ def ops_main(args) -> None:
         return torch.empty(rows, cols, device=dev).normal_(generator=gen).to(dtype)
 
     bf16, f32 = torch.bfloat16, torch.float32
-    print(f"{args.reps} calls each; GB/s over the bytes the operator cannot do without (every row named read or written once)\n")
-    print("| operator | shape | us per call | MB | GB/s | kernels (us) |")
-    print("|---|---|---|---|---|---|")
+    F, dense = torch.nn.functional, torch.ops.aten.embedding_dense_backward
+    print(f"{args.reps} calls each, shortest of three runs; GB/s over the bytes the operator cannot do without (every row "
+          "named read or written once)\n")
+    print("| operator | shape | us per call | MB | GB/s | PyTorch's calls (us) | kernels (us) |")
+    print("|---|---|---|---|---|---|---|")
 
-    def row(name, shape, fn, nbytes, kernels):
+    def per_call(fn):
         for _ in range(5):
             fn()
-        _lib.check(L.nbo_sync())
-        t0 = time.perf_counter()
-        for _ in range(args.reps):
-            fn()
-        _lib.check(L.nbo_sync())
-        us = (time.perf_counter() - t0) / args.reps * 1e6
+        best = 0.0
+        for _ in range(3):
+            torch.cuda.synchronize()
+            t0 = time.perf_counter()
+            for _ in range(args.reps):
+                fn()
+            torch.cuda.synchronize()
+            us = (time.perf_counter() - t0) / args.reps * 1e6
+            best = min(best, us) if best else us
+        return best
+
+    def row(name, shape, fn, nbytes, kernels, theirs):
+        us, torch_us = per_call(fn), per_call(theirs)
         _lib.check(L.nbo_profile_enable(1))
         for _ in range(args.reps):
             fn()
@@ -354,7 +364,8 @@ def ops_main(args) -> None:
             if cnt.value:
                 parts.append(f"`{k}` {ms.value / args.reps * 1e3:.1f}")
         _lib.check(L.nbo_profile_enable(0))
-        print(f"| {name} | {shape} | {us:.1f} | {nbytes / 1e6:.2f} | {nbytes / us / 1e3:.0f} | {', '.join(parts)} |", flush=True)
+        print(f"| {name} | {shape} | {us:.1f} | {nbytes / 1e6:.2f} | {nbytes / us / 1e3:.0f} | {torch_us:.1f} | {', '.join(parts)} |",
+              flush=True)
 
     order = ["nbo_embed_clear", "nbo_order_range", "nbo_order_split", "nbo_order_merge"]
     for rows, cols, n, dtype, tag, gdtype, gtag in ((128256, 4096, 1, bf16, "bf16", bf16, "bf16"),
@@ -367,15 +378,22 @@ def ops_main(args) -> None:
         shape = f"{n} of {rows} x {cols}"
         table, out = rand(rows, cols, dtype), rand(n, cols, dtype)
         row(f"embedding {tag}", shape, lambda: ops.embedding(table, ids, out), n * 8 + (named + n) * cols * size,
-            [f"nbo_embed_{tag}"])
+            [f"nbo_embed_{tag}"], lambda: F.embedding(ids, table))
+        if dtype == f32:
+            half = out.to(bf16)
+            row("embedding f32 -> bf16", shape, lambda: ops.embedding(table, ids, half), n * 8 + (2 * named + n) * cols * 2,
+                ["nbo_embed_f32_bf16"], lambda: F.embedding(ids, table).to(bf16))
         grad = table if gdtype == dtype else rand(rows, cols, gdtype)
         ws = ops.EmbeddingWorkspace(n, cols)
         kernels = order + [f"nbo_embed_{k}_{gtag}" for k in ("sum", "join", "direct")]
+        wide = (lambda: out) if gdtype == dtype else (lambda: out.to(gdtype))
         for accumulate in (False, True):
             row(f"embedding_grad {gtag}{' accumulate' if accumulate else ''}", shape,
                 lambda: ops.embedding_grad(out, ids, grad, ws, accumulate=accumulate),
-                n * 8 + n * cols * size + (2 * named if accumulate else rows) * cols * gsize, kernels)
-        del table, out, grad, ws
+                n * 8 + n * cols * size + (2 * named if accumulate else rows) * cols * gsize, kernels,
+                (lambda: grad.add_(dense(wide(), ids, rows, -1, False))) if accumulate else
+                (lambda: dense(wide(), ids, rows, -1, False)))
+        del table, out, grad, ws, wide
         torch.cuda.empty_cache()
     rng = ops.DropoutRng(1)
     for rows, cols, dtype, tag in ((32, 768, bf16, "bf16"), (8192, 768, f32, "f32"), (32768, 4096, bf16, "bf16")):
@@ -384,7 +402,8 @@ def ops_main(args) -> None:
         for residual in (None, r):
             row(f"dropout {tag}{' + residual' if residual is not None else ''}", f"{rows} x {cols}",
                 lambda: ops.dropout(x, 0.1, rng, 0, out, residual=residual),
-                x.numel() * dtype.itemsize * (2 if residual is None else 3), [f"nbo_dropout_{tag}"])
+                x.numel() * dtype.itemsize * (2 if residual is None else 3), [f"nbo_dropout_{tag}"],
+                lambda: F.dropout(x, 0.1) if residual is None else residual + F.dropout(x, 0.1))
         del x, r, out
         torch.cuda.empty_cache()
 
