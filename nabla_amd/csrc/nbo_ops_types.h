@@ -75,8 +75,9 @@ struct NboRngAdvanceArgs {
 // Split and merge: ids per tile, and the most keys of a range (LDS of the merge: 4 bytes for each wave and key).
 #define NBO_SPLIT_TILE 1024u
 #define NBO_SPLIT_KEYS 512u
-// Up to this many ids the gradient is one launch that needs no order (every workgroup holds all ids in registers;
-// 512 f32 rows of 3 KiB 6.6 us, 513 by way of an order 14.1).
+// Up to this many ids the gradient is one launch that needs no order: as many as every workgroup holds in eight
+// registers a lane.  That is the limit, and not where the two ways take the same time: 512 f32 rows of 3 KiB
+// 6.6 us, 513 by way of an order 14.1.
 #define NBO_EMBED_DIRECT_MAX 512u
 
 // Rows are dealt out to ranges: row v is number v >> shift of range v % 2^shift.
