@@ -21,10 +21,11 @@ clip + update + zeroing in one kernel (`fused_step_norm`); with a scaler *and* a
 the two decisions stay separate entry points in the reference's order.
 
 A generator given with `with_rng` (nabla_amd.ops.DropoutRng) is advanced once per micro-batch,
-whatever became of it, so that the dropouts of the next one draw other masks; its step is
-`state.rng_state`, its seed `state.rng_seed`, and checkpoints carry both (checkpoint.rs:107-150, `rng.state`;
-`rng.seed` is a line of this library's own).  The device has the only copy: whatever else advances or loads the generator, a replayed graph among it, a checkpoint has
-the step that the next mask is drawn with.
+whatever became of it, so that the dropouts of the next one draw other masks (a captured forward and
+backward pass leaves the advance to the tail).  Its step is `state.rng_state`, its seed `state.rng_seed`,
+and checkpoints carry both (checkpoint.rs:107-150, `rng.state`; `rng.seed` is a line of this library's
+own).  The device has the only copy: whatever else advances or loads the generator, a replayed graph
+among it, a checkpoint has the step that the next mask is drawn with.
 """
 from __future__ import annotations
 
